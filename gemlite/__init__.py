@@ -2,7 +2,7 @@
 
 Callers of the reference (`import gemlite`, `from gemlite.core import GemLiteLinearTriton`,
 `from gemlite.helper import A16W4_HQQ_INT`, external packages such as hqq) bind here without a change;
-`gemlite.core`, `.helper`, `.bitpack`, `.dtypes` and `.quant_utils` are the modules of `gemlite_b200` themselves,
+`gemlite.core`, `.helper`, `.bitpack`, `.dtypes`, `.quant_utils` and `.kv_cache` are the modules of `gemlite_b200` themselves,
 not copies, so state such as the config cache is shared whichever name was imported.  The export list is the
 reference's (gemlite/__init__.py:5-32).  There is no Triton code behind it: `gemlite.triton_kernels.config` only
 keeps the two objects that callers of the reference poke (`KERNEL_CACHE`, `set_autotune`)."""
@@ -20,7 +20,7 @@ from gemlite_b200 import (DType, GemLiteLinear, GemLiteLinearTriton, GEMLITE_ACC
 
 __version__ = _impl.__version__
 
-for _name in ("core", "helper", "bitpack", "dtypes", "quant_utils"):
+for _name in ("core", "helper", "bitpack", "dtypes", "quant_utils", "kv_cache"):
     _mod = importlib.import_module("gemlite_b200." + _name)
     sys.modules[__name__ + "." + _name] = _mod
     globals()[_name] = _mod

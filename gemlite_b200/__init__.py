@@ -26,6 +26,7 @@ from .core import (
     get_default_cache_config,
 )
 from . import helper
+from .kv_cache import KVBatch, QuantizedKVCache, rotary_table
 
 
 def auto_detect_ptx_fp4_pack():

@@ -42,6 +42,20 @@ class GLTpComm(ctypes.Structure):
                 ("buffers", c_void_p * 8)]
 
 
+class GLKvArgs(ctypes.Structure):
+    """Mirror of ``struct gl_kv_args``."""
+    _fields_ = [(n, c_void_p) for n in ("k_codes", "v_codes", "k_scales", "v_scales", "k_zeros", "v_zeros", "page_table", "lens",
+                                        "q_offsets", "q", "k", "v", "out", "out_v", "q_norm", "k_norm", "cos_sin", "positions",
+                                        "mask", "workspace")] + \
+               [("workspace_bytes", c_uint64)] + \
+               [(n, c_int64) for n in ("page_table_stride", "mask_stride", "q_stride_n", "q_stride_h", "k_stride_n", "k_stride_h",
+                                       "v_stride_n", "v_stride_h")] + \
+               [(n, c_int32) for n in ("format", "num_pages", "page_size", "n_kv_heads", "n_q_heads", "head_dim", "batch", "max_pages",
+                                       "n_tokens", "max_len", "max_new", "x_dtype", "norm_dtype", "rot_dim", "interleaved",
+                                       "table_rows", "mask_cols")] + \
+               [("eps", ctypes.c_float), ("softmax_scale", ctypes.c_float), ("kernel_override", c_int32)]
+
+
 # name -> (restype, argtypes); every symbol include/gemlite_b200.h declares
 SIGNATURES = {
     "gl_abi_version": (c_int32, []),
@@ -78,6 +92,10 @@ SIGNATURES = {
     "gl_tp_allreduce": (c_int32, [ctypes.POINTER(GLTpComm), c_void_p, c_void_p, c_int64, c_int32, c_int32, c_void_p]),
     "gl_tp_status": (c_int32, [ctypes.POINTER(GLTpComm), ctypes.POINTER(c_int32), ctypes.POINTER(ctypes.c_uint32)]),
     "gl_silu_mul": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p]),
+    "gl_kv_write": (c_int32, [ctypes.POINTER(GLKvArgs), c_void_p]),
+    "gl_kv_read": (c_int32, [ctypes.POINTER(GLKvArgs), c_void_p]),
+    "gl_kv_attend_workspace_bytes": (c_uint64, [ctypes.POINTER(GLKvArgs)]),
+    "gl_kv_attend": (c_int32, [ctypes.POINTER(GLKvArgs), c_void_p]),
     "gl_mma_peak": (c_int32, [c_int32, c_int32, c_void_p, ctypes.POINTER(ctypes.c_double), c_void_p]),
 }
 

@@ -296,6 +296,74 @@ GL_API int gl_tp_status(const gl_tp_comm* c, int32_t* status, uint32_t* epoch);
  * and the down projection of a decoder MLP (two torch ops in a host that runs the reference). fp16 / bf16. */
 GL_API int gl_silu_mul(const void* gate_up, void* out, int32_t M, int32_t inter, int32_t dtype, void* stream);
 
+/* ---- quantised key/value cache ------------------------------------------------------------------- */
+/* A paged cache of keys and values in low bits, written from the fused qkv projection's output and read by the attention
+ * kernel without being expanded in memory.  No counterpart in the reference (its layers end at the projections).
+ *
+ * Cache layout (all contiguous): codes [num_pages, n_kv_heads, page_size, row], row = head_dim bytes (GL_KV_FP8 e4m3,
+ * GL_KV_INT8) or head_dim / 2 bytes (GL_KV_INT4, even channel in the low nibble); scales fp32 [num_pages, n_kv_heads,
+ * page_size], positive; GL_KV_INT4: zeros uint8 of the same shape, 0..15.  value = (code - zero) * scale.  Codes are
+ * 16-byte aligned; head_dim is 64 or 128.
+ *
+ * Batch: sequence b holds lens[b] tokens already (gl_kv_read: the tokens to read); its new tokens are rows
+ * q_offsets[b] .. q_offsets[b+1] of the token-major operands (q_offsets NULL: n_tokens / batch rows each), its token p
+ * lives in page page_table[b, p / page_size].  Rows behind the last sequence's are neither read nor written.  A page
+ * number outside 0 .. num_pages - 1, or a token behind the table's last column, counts as absent: not written, not seen,
+ * read as zeros.  max_len and max_new are bounds of the lengths that the host knows; they shape the launch, results do
+ * not depend on them.
+ *
+ * Pointers and strides: q / k / v [n_tokens, heads, head_dim], fp16 or bf16, 16-byte aligned, strides in elements and
+ * multiples of 8, channels contiguous; outputs contiguous. */
+enum { GL_KV_FP8 = 0, GL_KV_INT8 = 1, GL_KV_INT4 = 2 };
+typedef struct gl_kv_args {
+  void*          k_codes;
+  void*          v_codes;
+  float*         k_scales;
+  float*         v_scales;
+  uint8_t*       k_zeros;       /* GL_KV_INT4, else NULL */
+  uint8_t*       v_zeros;
+  const int32_t* page_table;    /* [batch, max_pages], rows page_table_stride apart */
+  const int32_t* lens;          /* [batch] */
+  const int32_t* q_offsets;     /* [batch + 1] ascending, or NULL */
+  const void*    q;
+  const void*    k;
+  const void*    v;
+  void*          out;           /* write: rotated q; read: keys; attend: result */
+  void*          out_v;         /* read: values */
+  const void*    q_norm;        /* write: weights of the head norms [head_dim] (norm_dtype), or NULL */
+  const void*    k_norm;
+  const float*   cos_sin;       /* write: [table_rows, rot_dim], cosines then sines, or NULL */
+  const int32_t* positions;     /* write: [n_tokens], row of cos_sin */
+  const uint8_t* mask;          /* attend: [n_tokens, mask_cols], rows mask_stride apart, or NULL */
+  void*          workspace;     /* attend: gl_kv_attend_workspace_bytes(), 16-byte aligned, any content */
+  uint64_t       workspace_bytes;
+  int64_t        page_table_stride, mask_stride;
+  int64_t        q_stride_n, q_stride_h, k_stride_n, k_stride_h, v_stride_n, v_stride_h;
+  int32_t        format, num_pages, page_size, n_kv_heads, n_q_heads, head_dim;
+  int32_t        batch, max_pages, n_tokens, max_len, max_new;
+  int32_t        x_dtype;       /* q / k / v (write, attend); outputs of gl_kv_read (FP16 / BF16 / FP32) */
+  int32_t        norm_dtype, rot_dim, interleaved, table_rows, mask_cols;
+  float          eps, softmax_scale;
+  int32_t        kernel_override; /* attend: 0 = library picks, 1 = the mma.sync kernel, 2 = the tcgen05 kernel (testing / tuning) */
+} gl_kv_args;
+/* Queries and keys: head norm x / sqrt(mean x^2 + eps) * w (where weights are given), then the rotation of the first rot_dim
+ * channels (pairs i, i + rot_dim / 2, or 2i, 2i + 1 when interleaved) by row positions[n] of cos_sin; rot_dim is 0 or a
+ * multiple of 16.  Queries are rounded to x_dtype into `out` [n_tokens, n_q_heads, head_dim]; keys and values are quantised
+ * from fp32 into the cache: FP8 / INT8 scale = max(amax / qmax, 1e-6), code = round(x / scale) (half to even);
+ * INT4 over lo = min(0, min x), hi = max(0, max x): scale = max((hi - lo) / 15, 1e-6), zero = round(-lo / scale), code =
+ * clamp(round(x / scale) + zero, 0, 15).  A row (one token's head) that holds an infinity or NaN gets codes 0 and the
+ * scale NaN.  A position outside the table makes the token's queries NaN and its keys such a row.  A page that is written
+ * belongs to one sequence.  q may be NULL (n_q_heads is then ignored): only the cache is written. */
+GL_API int gl_kv_write(const gl_kv_args* a, void* stream);
+/* keys -> out, values -> out_v, [batch, max_len, n_kv_heads, head_dim] in x_dtype; zeros from lens[b] on. */
+GL_API int gl_kv_read(const gl_kv_args* a, void* stream);
+/* out[n, h] = sum_p softmax_p(softmax_scale * q[n, h] . K[p, h / group]) V[p, h / group] over what the token sees: the lens[b]
+ * cached tokens of its sequence, and of its sequence's new tokens (whose keys and values gl_kv_write has put behind them)
+ * those with mask[n, j] != 0, j < mask_cols, or, without a mask, those up to itself.  A row that sees nothing gives zeros.
+ * What a token does not see has no influence, whatever the bytes there hold. */
+GL_API uint64_t gl_kv_attend_workspace_bytes(const gl_kv_args* a);
+GL_API int gl_kv_attend(const gl_kv_args* a, void* stream);
+
 /* ---- measurement: tensor-pipe ceiling ------------------------------------------------------------ */
 /* Enqueues one kernel in which every SM issues iters x 4 tcgen05.mma of 128 x 256 x (32 bytes of K) on operand tiles
  * resident in shared memory: the MMA-issue ceiling for `kind` (GL_BF16, GL_FP8, GL_INT8, GL_MXFP4, GL_NVFP4) on this
