@@ -10,8 +10,9 @@
 // numbers).  q is fp16 already or is brought there from bf16 by a power of two per row (its largest channel lands in
 // [1, 2): channels 2^-14 of it and smaller lose bits, at most 2^-25 of the largest each).  P carries a factor 2^15, which
 // leaves the fp16 format 39 binary orders below the largest weight before a weight is lost.
-#include "gl_kv.cuh"
 #include "gl_kv_attend.cuh"
+#include <mutex>
+#include <vector>
 
 namespace {
 
@@ -19,7 +20,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kTinyScale = 1e-30f;
 constexpr int kTile = 32;          // tokens that a warp takes at a time
 constexpr int kWarps = 4;
-constexpr int kStages = 3;
+constexpr int kStages = 2;
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) { return __byte_perm(a, b, s); }
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -50,13 +51,13 @@ template <int RB> __device__ __forceinline__ uint32_t v_place(uint32_t t, uint32
 template <int D, int FMT> struct Shape {
   static constexpr int RB = FMT == GL_KV_INT4 ? D / 2 : D;         // bytes of a token's row
   static constexpr int CODES = kTile * RB;
-  static constexpr int K_AT = 0, V_AT = CODES, KS_AT = 2 * CODES, VS_AT = KS_AT + kTile * 4, KZ_AT = VS_AT + kTile * 4, VZ_AT = KZ_AT + kTile,
-                       VALID_AT = VZ_AT + kTile, STAGE = VALID_AT + 64;
+  static constexpr int K_AT = 0, V_AT = CODES, KS_AT = 2 * CODES, VS_AT = KS_AT + kTile * 4, RV_AT = VS_AT + kTile * 4, KZ_AT = RV_AT + kTile * 4,
+                       VZ_AT = KZ_AT + kTile, VALID_AT = VZ_AT + kTile, STAGE = VALID_AT + 64;
   static constexpr int LOOP = kWarps * kStages * STAGE;
 };
 
 template <int D, int FMT, int MT, typename T>
-__global__ void __launch_bounds__(kWarps * 32) kv_attend_mma_kernel(const KvAttendParams p) {
+__global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 3 : 2) kv_attend_mma_kernel(const KvAttendParams p) {
   using S = Shape<D, FMT>;
   constexpr int RB = S::RB, CPT = RB / 16, NT = D / 8, KS = D / 16, ROWS = 16 * MT;
   constexpr float kShift = 15.f;
@@ -66,24 +67,18 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_mma_kernel(const KvAtte
   gl_launch_dependents();
   gl_grid_dependency_wait();
 
-  const int b = blockIdx.z, kvh = blockIdx.y % kb.hkv, rt_step = gridDim.y / kb.hkv;
-  int first, end;
-  kv_new_rows(kb, b, first, end);
-  const int new_b = end - first;
-  if (new_b <= 0) return;
-  const int ctx = kv_len(kb, b);
-  const int len = (int)min((int64_t)ctx + new_b, kv_capacity(kb));
-  const int rows = new_b * p.group;
-  const int chunk = kv_attend_chunk(p, len);
-  const int c0 = blockIdx.x * chunk;
+  __shared__ KvPlaceScratch place_scratch;
+  KvWalk<ROWS> walk;
+  walk.start(p, kv_place_of_block<ROWS, kWarps * 32>(p, blockIdx.x, place_scratch), blockIdx.x);
 
   uint8_t* ring = smem + warp * kStages * S::STAGE;
   const uint32_t ring_u = smem_addr(ring);
 
-  for (int rt = blockIdx.y / kb.hkv; rt * ROWS < rows; rt += rt_step) {
-    const int r_base = rt * ROWS;
-    const int t_hi = min(new_b - 1, (r_base + ROWS - 1) / p.group);
-    const int c1 = min(min(c0 + chunk, len), p.mask == nullptr ? ctx + t_hi + 1 : len);
+  KvPiece pc;
+  while (walk.next(p, blockIdx.x, pc)) {
+    const int first = pc.s.first, ctx = pc.s.ctx, rows = pc.rows, kvh = pc.head;
+    const int c0 = pc.t0 * kKvTile, c1 = min(pc.t1 * kKvTile, pc.s.len);
+    const int64_t pt_row = (int64_t)walk.b * kb.pt_stride;
 
     // ---- queries as the A operand, channels in the order in which the codes come out of their words
     uint32_t qa[MT][KS][4];
@@ -93,9 +88,8 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_mma_kernel(const KvAtte
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        const int r = r_base + m * 16 + g + hf * 8;
-        const bool live = r < rows;
-        const int t = live ? r / p.group : 0, head = kvh * p.group + (live ? r - t * p.group : 0);
+        const bool live = m * 16 + g + hf * 8 < rows;
+        const int r = pc.row0 + (live ? m * 16 + g + hf * 8 : 0), t = r / p.group, head = kvh * p.group + (r - t * p.group);
         q_tok[m][hf] = t;
         const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)(first + t) * p.q_sn + (int64_t)head * p.q_sh;
         uint32_t w[D / 8];                                // this lane's D / 4 channels
@@ -155,7 +149,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_mma_kernel(const KvAtte
       const int pos = c0 + (warp + i * kWarps) * kTile + lane;
       if (i >= mine || pos >= c1) return -1;
       const int pi = p.page_shift >= 0 ? pos >> p.page_shift : pos / kb.page_size;
-      const int page = kb.page_table[b * kb.pt_stride + pi];
+      const int page = kb.page_table[pt_row + pi];
       if ((unsigned)page >= (unsigned)kb.num_pages) return -1;
       return ((int64_t)page * kb.hkv + kvh) * kb.page_size + (pos - pi * kb.page_size);
     };
@@ -176,6 +170,16 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_mma_kernel(const KvAtte
         const uint32_t at = ring_u + st * S::STAGE;
         const int64_t slot = slot_next;
         slot_next = slot_of(i + 1);
+        const int64_t slot0 = __shfl_sync(0xffffffffu, slot, 0);
+        if (__all_sync(0xffffffffu, slot == slot0 + lane && slot0 >= 0)) {         // 32 rows in a row: a tile inside one page
+          const uint8_t *ks = p.k_codes + slot0 * RB + lane * 16, *vs = p.v_codes + slot0 * RB + lane * 16;
+#pragma unroll
+          for (int k = 0; k < CPT; ++k) {
+            const int t = lane / CPT + k * (32 / CPT), ch = lane % CPT;
+            cp_async16(at + S::K_AT + k_place<RB>(t, ch), ks + k * 512, true);
+            cp_async16(at + S::V_AT + v_place<RB>(t, ch), vs + k * 512, true);
+          }
+        } else
 #pragma unroll
         for (int k = 0; k < CPT; ++k) {
           const int t = lane / CPT + k * (32 / CPT), ch = lane % CPT;
@@ -207,13 +211,15 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_mma_kernel(const KvAtte
       const int tile0 = c0 + (warp + i * kWarps) * kTile;
       const uint32_t there = *reinterpret_cast<const uint32_t*>(st + S::VALID_AT);
       const bool whole = there == 0xffffffffu && tile0 + kTile <= ctx;
-      // Rows of values that the sums cannot take as they are, lane = token.  A scale of (about) zero: log2 would leave no
-      // denominator, so the codes become zeros under a scale that does.  e4m3's NaN among new tokens: 0 * NaN would reach
-      // rows that do not see the token, so its codes become zeros under the scale NaN, which only reaches rows that do.
-      const float vs_lane = *reinterpret_cast<const float*>(st + S::VS_AT + lane * 4);
+      // Lane = token: log2 and reciprocal of its value scale.  Rows of values that the sums cannot take as they are: a scale of
+      // (about) zero would leave no denominator, so the codes become zeros under a scale that does.  e4m3's NaN among new
+      // tokens: 0 * NaN would reach rows that do not see the token, so its codes become zeros under the scale NaN, which only
+      // reaches rows that do.
+      float vs_lane = *reinterpret_cast<const float*>(st + S::VS_AT + lane * 4);
       if (__any_sync(0xffffffffu, vs_lane < kTinyScale || (FMT == GL_KV_FP8 && !whole))) {
         bool nan = false;
         if (FMT == GL_KV_FP8 && !whole) {
+#pragma unroll 1
           for (int ch = 0; ch < CPT; ++ch) {
             const uint4 u = *reinterpret_cast<const uint4*>(st + S::V_AT + v_place<RB>(lane, ch));
             const uint32_t m = 0x7f7f7f7fu, one = 0x01010101u;
@@ -221,12 +227,15 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_mma_kernel(const KvAtte
           }
         }
         if (nan || vs_lane < kTinyScale) {
+#pragma unroll 1
           for (int ch = 0; ch < CPT; ++ch) *reinterpret_cast<uint4*>(st + S::V_AT + v_place<RB>(lane, ch)) = make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<float*>(st + S::VS_AT + lane * 4) = nan ? __int_as_float(0x7fc00000) : kTinyScale;
+          vs_lane = nan ? __int_as_float(0x7fc00000) : kTinyScale;
           if (FMT == GL_KV_INT4) st[S::VZ_AT + lane] = 0;
         }
-        __syncwarp();
       }
+      *reinterpret_cast<float*>(st + S::VS_AT + lane * 4) = __log2f(vs_lane);
+      *reinterpret_cast<float*>(st + S::RV_AT + lane * 4) = __frcp_rn(vs_lane);
+      __syncwarp();
 
       // ---- scores
       float s[MT][4][4];
@@ -267,20 +276,16 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_mma_kernel(const KvAtte
       }
 
       // ---- exponents
-      float rv[4][2];
 #pragma unroll
       for (int nt = 0; nt < 4; ++nt) {
         const float2 ks = *reinterpret_cast<const float2*>(st + S::KS_AT + (nt * 8 + 2 * c) * 4);
-        const float2 vs = *reinterpret_cast<const float2*>(st + S::VS_AT + (nt * 8 + 2 * c) * 4);
-        const float lx = __log2f(vs.x), ly = __log2f(vs.y);
-        rv[nt][0] = __frcp_rn(vs.x);
-        rv[nt][1] = __frcp_rn(vs.y);
+        const float2 lv = *reinterpret_cast<const float2*>(st + S::VS_AT + (nt * 8 + 2 * c) * 4);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          s[m][nt][0] = fmaf(s[m][nt][0] * ks.x, qs[m][0], lx);
-          s[m][nt][1] = fmaf(s[m][nt][1] * ks.y, qs[m][0], ly);
-          s[m][nt][2] = fmaf(s[m][nt][2] * ks.x, qs[m][1], lx);
-          s[m][nt][3] = fmaf(s[m][nt][3] * ks.y, qs[m][1], ly);
+          s[m][nt][0] = fmaf(s[m][nt][0] * ks.x, qs[m][0], lv.x);
+          s[m][nt][1] = fmaf(s[m][nt][1] * ks.y, qs[m][0], lv.y);
+          s[m][nt][2] = fmaf(s[m][nt][2] * ks.x, qs[m][1], lv.x);
+          s[m][nt][3] = fmaf(s[m][nt][3] * ks.y, qs[m][1], lv.y);
         }
       }
       if (!whole) {
@@ -325,10 +330,15 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_mma_kernel(const KvAtte
         const float sub0 = top[0] == -INFINITY ? 0.f : top[0] - kShift, sub1 = top[1] == -INFINITY ? 0.f : top[1] - kShift;
 #pragma unroll
         for (int nt = 0; nt < 4; ++nt) {
+          const float2 rv = *reinterpret_cast<const float2*>(st + S::RV_AT + (nt * 8 + 2 * c) * 4);
           const float e0 = kv_exp2(s[m][nt][0] - sub0), e1 = kv_exp2(s[m][nt][1] - sub0), e2 = kv_exp2(s[m][nt][2] - sub1), e3 = kv_exp2(s[m][nt][3] - sub1);
-          // a token that is not seen has the weight 0, also where its scale is NaN
-          sum[m][0] += (whole || s[m][nt][0] != -INFINITY ? e0 * rv[nt][0] : 0.f) + (whole || s[m][nt][1] != -INFINITY ? e1 * rv[nt][1] : 0.f);
-          sum[m][1] += (whole || s[m][nt][2] != -INFINITY ? e2 * rv[nt][0] : 0.f) + (whole || s[m][nt][3] != -INFINITY ? e3 * rv[nt][1] : 0.f);
+          if (whole) {
+            sum[m][0] = fmaf(e0, rv.x, fmaf(e1, rv.y, sum[m][0]));
+            sum[m][1] = fmaf(e2, rv.x, fmaf(e3, rv.y, sum[m][1]));
+          } else {                                         // a token that is not seen has the weight 0, also where its scale is NaN
+            sum[m][0] += (s[m][nt][0] != -INFINITY ? e0 * rv.x : 0.f) + (s[m][nt][1] != -INFINITY ? e1 * rv.y : 0.f);
+            sum[m][1] += (s[m][nt][2] != -INFINITY ? e2 * rv.x : 0.f) + (s[m][nt][3] != -INFINITY ? e3 * rv.y : 0.f);
+          }
           const __half2 lo = __floats2half2_rn(e0, e1), hi = __floats2half2_rn(e2, e3);
           pa[m][nt >> 1][(nt & 1) * 2] = *reinterpret_cast<const uint32_t*>(&lo);
           pa[m][nt >> 1][(nt & 1) * 2 + 1] = *reinterpret_cast<const uint32_t*>(&hi);
@@ -417,7 +427,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_mma_kernel(const KvAtte
     __syncthreads();
     for (int at = tid * 4; at < ROWS * D; at += kWarps * 32 * 4) {
       const int r = at / D, d = at % D;
-      if (r_base + r >= rows) break;
+      if (r >= rows) break;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
       float top = -INFINITY, l = 0.f;
 #pragma unroll
@@ -429,127 +439,140 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_mma_kernel(const KvAtte
         const float2 m2 = ml[w * ROWS + r];
         l += m2.x == -INFINITY ? 0.f : m2.y * kv_exp2(m2.x - top);
       }
-      const int rr = r_base + r, t = rr / p.group;
-      const int64_t row = (int64_t)(first + t) * p.hq + kvh * p.group + (rr - t * p.group);
-      if (p.splits > 1) {
-        const int64_t pr = (int64_t)blockIdx.x * kb.n_tokens * p.hq + row;
-        if (l != 0.f) *reinterpret_cast<float4*>(p.part_o + pr * D + d) = acc;     // (NaN is not 0)
-        if (d == 0) p.part_ml[pr] = make_float2(top, l);
+      const int rr = pc.row0 + r, t = rr / p.group;
+      if (pc.whole) {
+        kv_store4<T>(reinterpret_cast<T*>(p.out) + ((int64_t)(first + t) * p.hq + kvh * p.group + (rr - t * p.group)) * D + d, acc, l);
       } else {
-        kv_store4<T>(reinterpret_cast<T*>(p.out) + row * D + d, acc, l);
+        const int64_t pr = (int64_t)pc.slot * ROWS + r;
+        *reinterpret_cast<float4*>(p.part_o + pr * D + d) = acc;
+        if (d == 0) p.part_ml[pr] = make_float2(top, l);
       }
     }
     __syncthreads();
   }
 }
 
-// Joins the parts of a split sequence: one block per row, warp w takes splits w, w + 8, ..
-template <int D, typename T>
+// Joins the parts of the units that block borders cut.  Block (i, y) looks after border i + 1 if it is the first one in its
+// unit: rows y, y + gridDim.y, .., warp w takes parts w, w + 8, ..
+template <int ROWS, int D, typename T>
 __global__ void __launch_bounds__(256) kv_attend_join_kernel(const KvAttendParams p) {
+  __shared__ KvPlaceScratch place_scratch;
   __shared__ float4 acc_s[8][D / 4];
   __shared__ float red[8];
-  const int64_t row = blockIdx.x, rows = (int64_t)p.kb.n_tokens * p.hq;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = (int)(row / p.hq);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, border = blockIdx.x + 1;
   gl_launch_dependents();
   gl_grid_dependency_wait();
-  // rows that belong to no sequence stay as they were
-  if (p.kb.q_offsets != nullptr && (n < p.kb.q_offsets[0] || n >= p.kb.q_offsets[p.kb.batch])) return;
+  const KvPlace pl = kv_place_of_block<ROWS, 256>(p, border, place_scratch);
+  if (pl.b < 0) return;
+  const KvSeq s = kv_seq<ROWS>(p, pl.b);
+  const int u = (int)kv_div(pl.off, s.tiles);
+  const int64_t begin = pl.prefix + (int64_t)u * s.tiles;
+  if (begin == pl.prefix + pl.off) return;                       // the border is the unit's own
+  const KvShare share(pl.total, p.blocks);
+  const int i0 = share.owner(begin), i1 = share.owner(begin + s.tiles - 1);      // every block from i0 to i1 has tiles of the unit
+  if (i0 != border - 1) return;                                  // an earlier border of the unit does the work
+  const int head = u / s.blocks, row0 = kv_row_block(u - head * s.blocks, s.blocks) * ROWS, rows = min(ROWS, s.new_b * p.group - row0);
+  auto part = [&](int i) { return (int64_t)(2 * i + (i == i0 ? 1 : 0)) * ROWS; };
 
-  float top = -INFINITY;
-  for (int s = tid; s < p.splits; s += 256) {
-    const float2 ml = p.part_ml[s * rows + row];
-    if (ml.y != 0.f) top = fmaxf(top, ml.x);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) red[warp] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 8; ++w) top = fmaxf(top, red[w]);
-  __syncthreads();
-  constexpr int V = D / 32;
-  float acc[V] = {};
-  float l = 0.f;
-#pragma unroll 4
-  for (int s = warp; s < p.splits; s += 8) {
-    const float2 ml = p.part_ml[s * rows + row];
-    if (ml.y == 0.f) continue;
-    const float f = ml.x == -INFINITY ? ml.y : kv_exp2(ml.x - top);    // -inf with a sum: the sum is NaN
-    l += ml.y * f;
-    const float* src = p.part_o + (s * rows + row) * D + lane * V;
-#pragma unroll
-    for (int j = 0; j < V; ++j) acc[j] += src[j] * f;
-  }
-#pragma unroll
-  for (int j = 0; j < V; ++j) reinterpret_cast<float*>(acc_s[warp])[lane * V + j] = acc[j];
-  if (lane == 0) red[warp] = l;
-  __syncthreads();
-  if (tid < D / 4) {
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    l = 0.f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      const float4 x = acc_s[w][tid];
-      a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
-      l += red[w];
+  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+    float top = -INFINITY;
+    for (int i = i0 + tid; i <= i1; i += 256) {
+      const float2 ml = p.part_ml[part(i) + r];
+      if (ml.y != 0.f) top = fmaxf(top, ml.x);
     }
-    kv_store4<T>(reinterpret_cast<T*>(p.out) + row * D + tid * 4, a, l);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) red[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) top = fmaxf(top, red[w]);
+    __syncthreads();
+    constexpr int V = D / 32;
+    float acc[V] = {};
+    float l = 0.f;
+#pragma unroll 4
+    for (int i = i0 + warp; i <= i1; i += 8) {
+      const float2 ml = p.part_ml[part(i) + r];
+      if (ml.y == 0.f) continue;
+      const float f = ml.x == -INFINITY ? ml.y : kv_exp2(ml.x - top);    // -inf with a sum: the sum is NaN
+      l += ml.y * f;
+      const float* src = p.part_o + (part(i) + r) * D + lane * V;
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] += src[j] * f;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) reinterpret_cast<float*>(acc_s[warp])[lane * V + j] = acc[j];
+    if (lane == 0) red[warp] = l;
+    __syncthreads();
+    if (tid < D / 4) {
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+      l = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        const float4 x = acc_s[w][tid];
+        a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+        l += red[w];
+      }
+      const int rr = row0 + r, t = rr / p.group;
+      kv_store4<T>(reinterpret_cast<T*>(p.out) + ((int64_t)(s.first + t) * p.hq + head * p.group + (rr - t * p.group)) * D + tid * 4, a, l);
+    }
+    __syncthreads();
   }
 }
 
 template <int D, int FMT, int MT, typename T>
-int launch_mma(const KvAttendParams& p, dim3 grid, cudaStream_t st) {
+int launch_mma(const KvAttendParams& p, cudaStream_t st) {
   constexpr int LOOP = Shape<D, FMT>::LOOP, JOIN = kWarps * 16 * MT * (D * 4 + 8), SMEM = LOOP > JOIN ? LOOP : JOIN;
-  static bool set[64];
-  int dev = 0;
-  GL_CUDA_CHECK(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64 || !set[dev]) {
-    GL_CUDA_CHECK(cudaFuncSetAttribute(kv_attend_mma_kernel<D, FMT, MT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
-    if (dev >= 0 && dev < 64) set[dev] = true;
-  }
-  GL_CUDA_CHECK(gl_launch_pdl(kv_attend_mma_kernel<D, FMT, MT, T>, grid, dim3(kWarps * 32), SMEM, st, p));
+  if (int rc = kv_allow_smem((const void*)kv_attend_mma_kernel<D, FMT, MT, T>, SMEM)) return rc;
+  GL_CUDA_CHECK(gl_launch_pdl(kv_attend_mma_kernel<D, FMT, MT, T>, dim3((unsigned)p.blocks), dim3(kWarps * 32), SMEM, st, p));
   return GL_OK;
 }
 template <int D, int FMT, typename T>
-int launch_rows(const KvAttendParams& p, int mt, dim3 grid, cudaStream_t st) {
-  return mt == 1 ? launch_mma<D, FMT, 1, T>(p, grid, st) : launch_mma<D, FMT, 2, T>(p, grid, st);
+int launch_rows(const KvAttendParams& p, int mt, cudaStream_t st) {
+  return mt == 1 ? launch_mma<D, FMT, 1, T>(p, st) : launch_mma<D, FMT, 2, T>(p, st);
 }
 template <int D, typename T>
-int launch_fmt(const KvAttendParams& p, int fmt, int mt, dim3 grid, cudaStream_t st) {
+int launch_fmt(const KvAttendParams& p, int fmt, int mt, cudaStream_t st) {
   switch (fmt) {
-    case GL_KV_FP8: return launch_rows<D, GL_KV_FP8, T>(p, mt, grid, st);
-    case GL_KV_INT8: return launch_rows<D, GL_KV_INT8, T>(p, mt, grid, st);
-    default: return launch_rows<D, GL_KV_INT4, T>(p, mt, grid, st);
+    case GL_KV_FP8: return launch_rows<D, GL_KV_FP8, T>(p, mt, st);
+    case GL_KV_INT8: return launch_rows<D, GL_KV_INT8, T>(p, mt, st);
+    default: return launch_rows<D, GL_KV_INT4, T>(p, mt, st);
   }
 }
-template <typename T>
-int launch_mma_any(const KvAttendParams& p, int d, int fmt, int mt, dim3 grid, cudaStream_t st) {
-  return d == 128 ? launch_fmt<128, T>(p, fmt, mt, grid, st) : launch_fmt<64, T>(p, fmt, mt, grid, st);
+template <int ROWS, int D, typename T>
+int launch_join(const KvAttendParams& p, int live_rows, cudaStream_t st) {
+  const int y = live_rows < 64 ? live_rows : 64;
+  GL_CUDA_CHECK(gl_launch_pdl(kv_attend_join_kernel<ROWS, D, T>, dim3((unsigned)(p.blocks - 1), (unsigned)y), dim3(256), 0, st, p));
+  return GL_OK;
+}
+template <int D, typename T>
+int launch_all(const KvAttendParams& p, const gl_kv_args* a, int rows, int live_rows, cudaStream_t st) {
+  if (int rc = rows == kKvTcRows ? gl_kv_attend_tc_launch(p, D, a->format, a->x_dtype, st) : launch_fmt<D, T>(p, a->format, rows / 16, st)) return rc;
+  if (p.blocks == 1) return GL_OK;
+  if (rows == kKvTcRows) return launch_join<kKvTcRows, D, T>(p, live_rows, st);
+  return rows == 16 ? launch_join<16, D, T>(p, live_rows, st) : launch_join<32, D, T>(p, live_rows, st);
 }
 
 struct Plan {
-  int mt, row_tiles, splits, chunk;
+  int rows, live_rows, blocks;      // rows of a unit, the most of them that are live, thread blocks
 };
 
-// How the work is cut.  Tokens are the long axis: a (sequence, kv head, row tile) gets as many splits as fill the SMs
-// kWaves times over, none shorter than 128 tokens (one trip of the four warps).
+// Few rows per kv head: the mma.sync kernel, which holds 16 or 32 rows in registers (two blocks per SM); more: the tcgen05
+// kernel with 256 (one per SM).
 Plan plan_of(const gl_kv_args* a) {
   Plan pl;
   const int group = a->n_q_heads / a->n_kv_heads;
-  const int64_t max_rows = (int64_t)(a->max_new < a->n_tokens ? a->max_new : a->n_tokens) * group;
-  pl.mt = max_rows <= 16 ? 1 : 2;
-  int64_t tiles = gl_cdiv(max_rows, 16 * pl.mt);
-  const int64_t most = 65535 / a->n_kv_heads;
-  if (tiles > most) tiles = most;
-  pl.row_tiles = tiles < 1 ? 1 : (int)tiles;
+  int64_t max_rows = (int64_t)(a->max_new < a->n_tokens ? a->max_new : a->n_tokens) * group;
+  if (max_rows < 1) max_rows = 1;
+  const bool tc = a->kernel_override == 2 || (a->kernel_override == 0 && max_rows > 32);
+  pl.rows = tc ? kKvTcRows : max_rows <= 16 ? 16 : 32;
+  pl.live_rows = (int)(max_rows < pl.rows ? max_rows : pl.rows);
   const int64_t cap = (int64_t)a->max_pages * a->page_size;
   int64_t len = a->max_len < cap ? a->max_len : cap;
   if (len < 1) len = 1;
-  const int64_t units = (int64_t)a->batch * a->n_kv_heads * pl.row_tiles, want = gl_cdiv((int64_t)gl_num_sms() * 2 * 4, units);
-  int64_t chunk = gl_cdiv(gl_cdiv(len, want), 128) * 128;
-  const int64_t splits = gl_cdiv(len, chunk);
-  pl.splits = (int)(splits < 1024 ? splits : 1024);
-  pl.chunk = (int)(gl_cdiv(gl_cdiv(len, pl.splits), 128) * 128);
+  const int64_t work = (int64_t)a->batch * a->n_kv_heads * gl_cdiv(max_rows, pl.rows) * gl_cdiv(len, kKvTile);
+  const int64_t most = (int64_t)gl_num_sms() * (tc ? 1 : pl.rows == 16 ? 3 : 2);
+  pl.blocks = (int)(work < most ? work : most);
   return pl;
 }
 
@@ -557,18 +580,34 @@ int check_attend(const gl_kv_args* a) {
   if (int rc = gl_kv_check("gl_kv_attend", a)) return rc;
   if (a->x_dtype != GL_FP16 && a->x_dtype != GL_BF16) GL_FAIL(GL_E_UNSUPPORTED, "gl_kv_attend: dtype %d (fp16 / bf16 only)", a->x_dtype);
   if (a->n_q_heads <= 0 || a->n_q_heads % a->n_kv_heads != 0) GL_FAIL(GL_E_INVALID, "gl_kv_attend: %d query heads over %d kv heads", a->n_q_heads, a->n_kv_heads);
-  if (a->batch > 65535 || a->n_kv_heads > 65535) GL_FAIL(GL_E_UNSUPPORTED, "gl_kv_attend: %d sequences, %d kv heads (at most 65535)", a->batch, a->n_kv_heads);
+  if (a->kernel_override < 0 || a->kernel_override > 2) GL_FAIL(GL_E_INVALID, "gl_kv_attend: kernel_override %d", a->kernel_override);
+  // row numbers and tile counts of a sequence stay below 2^31, tiles in all times blocks below 2^63
   if ((int64_t)a->n_tokens * a->n_q_heads > 0x7fffffffll) GL_FAIL(GL_E_UNSUPPORTED, "gl_kv_attend: %d tokens of %d heads", a->n_tokens, a->n_q_heads);
   if ((int64_t)a->max_pages * a->page_size > 0x40000000ll) GL_FAIL(GL_E_UNSUPPORTED, "gl_kv_attend: page table of %d x %d tokens (at most 2^30)", a->max_pages, a->page_size);
   return GL_OK;
 }
 
 uint64_t workspace_of(const gl_kv_args* a, const Plan& pl) {
-  if (pl.splits <= 1) return 0;
-  return (uint64_t)pl.splits * (uint64_t)a->n_tokens * (uint64_t)a->n_q_heads * (uint64_t)(a->head_dim * 4 + 8);
+  if (pl.blocks <= 1) return 0;
+  return 2ull * (uint64_t)pl.blocks * (uint64_t)pl.rows * (uint64_t)(a->head_dim * 4 + 8);
 }
 
 }  // namespace
+
+int kv_allow_smem(const void* kernel, int bytes) {
+  // remembered per device and kernel; a kernel that is not found twice at the same time is set twice, which does no harm
+  struct Entry { const void* kernel; int dev; };
+  static std::mutex mu;
+  static std::vector<Entry> done;
+  int dev = 0;
+  GL_CUDA_CHECK(cudaGetDevice(&dev));
+  std::lock_guard<std::mutex> lk(mu);
+  for (const Entry& e : done)
+    if (e.kernel == kernel && e.dev == dev) return GL_OK;
+  GL_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.push_back({kernel, dev});
+  return GL_OK;
+}
 
 extern "C" uint64_t gl_kv_attend_workspace_bytes(const gl_kv_args* a) {
   if (check_attend(a) != GL_OK || a->batch == 0 || a->n_tokens == 0) return 0;
@@ -594,23 +633,12 @@ extern "C" int gl_kv_attend(const gl_kv_args* a, void* stream) {
   p.q_sn = a->q_stride_n; p.q_sh = a->q_stride_h; p.mask_stride = a->mask_stride;
   p.mask_cols = a->mask_cols; p.hq = a->n_q_heads; p.group = a->n_q_heads / a->n_kv_heads;
   p.scale_log2 = a->softmax_scale * kLog2e;
-  p.splits = pl.splits; p.chunk = pl.chunk;
+  p.blocks = pl.blocks;
   p.page_shift = (a->page_size & (a->page_size - 1)) == 0 ? __builtin_ctz((unsigned)a->page_size) : -1;
-  const int64_t rows = (int64_t)a->n_tokens * a->n_q_heads;
   p.part_o = (float*)a->workspace;
-  p.part_ml = need > 0 ? reinterpret_cast<float2*>(p.part_o + (int64_t)pl.splits * rows * a->head_dim) : nullptr;
+  p.part_ml = need > 0 ? reinterpret_cast<float2*>(p.part_o + 2ll * pl.blocks * pl.rows * a->head_dim) : nullptr;
   cudaStream_t st = (cudaStream_t)stream;
-  const dim3 grid((unsigned)pl.splits, (unsigned)(a->n_kv_heads * pl.row_tiles), (unsigned)a->batch);
-  const int rc = a->x_dtype == GL_BF16 ? launch_mma_any<__nv_bfloat16>(p, a->head_dim, a->format, pl.mt, grid, st)
-                                       : launch_mma_any<__half>(p, a->head_dim, a->format, pl.mt, grid, st);
-  if (rc != GL_OK || pl.splits == 1) return rc;
-  const dim3 jg((unsigned)rows);
-  if (a->head_dim == 128) {
-    if (a->x_dtype == GL_BF16) GL_CUDA_CHECK(gl_launch_pdl(kv_attend_join_kernel<128, __nv_bfloat16>, jg, dim3(256), 0, st, p));
-    else GL_CUDA_CHECK(gl_launch_pdl(kv_attend_join_kernel<128, __half>, jg, dim3(256), 0, st, p));
-  } else {
-    if (a->x_dtype == GL_BF16) GL_CUDA_CHECK(gl_launch_pdl(kv_attend_join_kernel<64, __nv_bfloat16>, jg, dim3(256), 0, st, p));
-    else GL_CUDA_CHECK(gl_launch_pdl(kv_attend_join_kernel<64, __half>, jg, dim3(256), 0, st, p));
-  }
-  return GL_OK;
+  if (a->head_dim == 128)
+    return a->x_dtype == GL_BF16 ? launch_all<128, __nv_bfloat16>(p, a, pl.rows, pl.live_rows, st) : launch_all<128, __half>(p, a, pl.rows, pl.live_rows, st);
+  return a->x_dtype == GL_BF16 ? launch_all<64, __nv_bfloat16>(p, a, pl.rows, pl.live_rows, st) : launch_all<64, __half>(p, a, pl.rows, pl.live_rows, st);
 }

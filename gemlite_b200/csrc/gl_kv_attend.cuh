@@ -9,22 +9,172 @@ struct KvAttendParams {
   const void* q;
   void* out;
   const uint8_t* mask;
-  float* part_o;               // [splits][n_tokens * hq][D], unnormalised
-  float2* part_ml;             // [splits][n_tokens * hq]: maximum and sum (0: nothing seen)
+  float* part_o;               // [2 * blocks][rows of a unit][D], unnormalised
+  float2* part_ml;             // [2 * blocks][rows of a unit]: maximum and sum (0: nothing seen)
   int64_t q_sn, q_sh, mask_stride;
-  int32_t mask_cols, hq, group, splits, chunk, page_shift;
+  int32_t mask_cols, hq, group, page_shift, blocks;
   float scale_log2;
 };
+
+// the tcgen05 kernel (gl_kv_attend_tc.cu): 256 query rows of a kv head per unit, one block per SM
+constexpr int kKvTcRows = 256;
+// opt-in to more than 48 KB of dynamic shared memory on the current device, once per kernel
+int kv_allow_smem(const void* kernel, int bytes);
+int gl_kv_attend_tc_launch(const KvAttendParams& p, int head_dim, int format, int x_dtype, cudaStream_t st);
 
 template <typename T> struct IsHalf { static constexpr bool value = false; };
 template <> struct IsHalf<__half> { static constexpr bool value = true; };
 
 #ifdef __CUDACC__
-// Tokens per split of a sequence: the launch's, or more where the sequence is longer than the host's bound said.
-__device__ __forceinline__ int kv_attend_chunk(const KvAttendParams& p, int len) {
-  const int need = (len + p.splits - 1) / p.splits;
-  return max(p.chunk, (need + 127) / 128 * 128);
+// ---- how the work is dealt out
+// A unit is ROWS query rows (token, head of the group) of one kv head of one sequence; it is worked through in tiles of kKvTile cached
+// tokens.  All units' tiles stand in one line (sequence, kv head, row block, tile), and block i of n takes the i-th of n
+// equal pieces of the line: lengths may differ as they like, every block gets the same number of tiles, and a unit is cut
+// only where a block ends.  A block whose piece holds a whole unit writes the unit's result; the part of a unit that it starts in
+// the middle of goes to its scratch slot 2 i, the part that it does not finish to slot 2 i + 1, and kv_attend_join_kernel joins.
+// Nobody waits for anybody.  The lengths are on the device, so every block adds them up for itself.
+constexpr int kKvTile = 128;
+
+struct KvSeq {
+  int first, new_b, ctx, len, tiles, blocks;      // blocks: row blocks per kv head (0: no new tokens)
+};
+template <int ROWS> __device__ __forceinline__ KvSeq kv_seq(const KvAttendParams& p, int b) {
+  KvSeq s;
+  int end;
+  kv_new_rows(p.kb, b, s.first, end);
+  s.new_b = end - s.first;
+  s.ctx = kv_len(p.kb, b);
+  s.len = (int)min((int64_t)s.ctx + s.new_b, kv_capacity(p.kb));
+  s.tiles = max(1, (s.len + kKvTile - 1) / kKvTile);
+  s.blocks = (int)(((int64_t)s.new_b * p.group + ROWS - 1) / ROWS);
+  return s;
 }
+__device__ __forceinline__ int64_t kv_seq_work(const KvAttendParams& p, const KvSeq& s) { return (int64_t)p.kb.hkv * s.blocks * s.tiles; }
+
+// 64-bit quotients of numbers that almost always have 32 (the general routine is a hundred instructions)
+__device__ __forceinline__ int64_t kv_div(int64_t a, int64_t b) {
+  return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+// the line's pieces: the first `more` blocks get `each` + 1 tiles, the others `each`
+struct KvShare {
+  int64_t total, each;
+  int more;
+  __device__ __forceinline__ KvShare(int64_t t, int blocks) : total(t), each(kv_div(t, blocks)), more((int)(t - each * blocks)) {}
+  __device__ __forceinline__ int64_t begin(int i) const { return each * i + min(i, more); }
+  // the block whose piece holds tile x < total
+  __device__ __forceinline__ int owner(int64_t x) const {
+    const int64_t y = x - more * (each + 1);
+    return (int)(y < 0 ? kv_div(x, each + 1) : more + kv_div(y, each));
+  }
+};
+// place in the line: sequence, and tiles of the sequence before it
+struct KvPlace {
+  int64_t total, prefix, off;      // tiles in all; tiles before the sequence; within it
+  int b;                           // -1: behind the end
+};
+struct KvPlaceScratch {
+  int64_t warp_sum[32];
+  int64_t prefix, off;
+  int b;
+};
+// Where block `i` of p.blocks begins (i = p.blocks: the end).  All THREADS threads of the block; ends with __syncthreads.
+template <int ROWS, int THREADS> __device__ __forceinline__ KvPlace kv_place_of_block(const KvAttendParams& p, int i, KvPlaceScratch& sc) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = p.kb.batch;
+  const int per = (B + THREADS - 1) / THREADS, lo = min(tid * per, B), hi = min(lo + per, B);
+  int64_t sum = 0;
+  for (int b = lo; b < hi; ++b) sum += kv_seq_work(p, kv_seq<ROWS>(p, b));
+  int64_t incl = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) sc.warp_sum[warp] = incl;
+  if (tid == 0) sc.b = -1;
+  __syncthreads();
+  int64_t before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += sc.warp_sum[w];
+    total += sc.warp_sum[w];
+  }
+  int64_t prefix = before + incl - sum;
+  const int64_t x = KvShare(total, p.blocks).begin(i);
+  if (x >= prefix && x < prefix + sum) {
+    for (int b = lo; b < hi; ++b) {
+      const int64_t w = kv_seq_work(p, kv_seq<ROWS>(p, b));
+      if (x < prefix + w) {
+        sc.b = b;
+        sc.prefix = prefix;
+        sc.off = x - prefix;
+        break;
+      }
+      prefix += w;
+    }
+  }
+  __syncthreads();
+  KvPlace pl;
+  pl.total = total;
+  pl.b = sc.b;
+  pl.prefix = sc.prefix;
+  pl.off = sc.off;
+  return pl;
+}
+// row blocks are taken from both ends in turn: without a mask, late ones see more tokens than early ones
+__device__ __forceinline__ int kv_row_block(int i, int n) { return (i & 1) ? n - 1 - (i >> 1) : i >> 1; }
+
+struct KvPiece {
+  KvSeq s;
+  int head, row0, rows;            // kv head; first row of the unit and its live rows
+  int t0, t1;                      // tiles of this piece that some row may see (t1 <= t0: none)
+  bool whole;                      // the unit's tiles are all in this piece
+  int slot;                        // else: scratch slot of its part
+};
+// walks a block's piece of the line, unit by unit
+template <int ROWS> struct KvWalk {
+  int b, left_valid;
+  int64_t off, left;               // place within sequence b; tiles left to take
+  bool at_start;
+  KvSeq s;
+  __device__ __forceinline__ void start(const KvAttendParams& p, const KvPlace& pl, int i) {
+    b = pl.b;
+    off = pl.off;
+    const KvShare share(pl.total, p.blocks);
+    left = b < 0 ? 0 : share.begin(i + 1) - share.begin(i);
+    left_valid = 0;
+  }
+  __device__ __forceinline__ bool next(const KvAttendParams& p, int i, KvPiece& pc) {
+    if (left <= 0) return false;
+    while (true) {
+      if (!left_valid) {
+        if (b >= p.kb.batch) return false;
+        s = kv_seq<ROWS>(p, b);
+        left_valid = 1;
+      }
+      if (off < kv_seq_work(p, s)) break;
+      ++b;
+      off = 0;
+      left_valid = 0;
+    }
+    const int u = (int)kv_div(off, s.tiles), t0 = (int)(off - (int64_t)u * s.tiles), t1 = (int)min((int64_t)s.tiles, t0 + left);
+    const int head = u / s.blocks, rb = kv_row_block(u - head * s.blocks, s.blocks);
+    off += t1 - t0;
+    left -= t1 - t0;
+    pc.s = s;
+    pc.head = head;
+    pc.row0 = rb * ROWS;
+    pc.rows = min(ROWS, s.new_b * p.group - pc.row0);
+    pc.whole = t0 == 0 && t1 == s.tiles;
+    pc.slot = 2 * i + (t0 == 0 ? 1 : 0);
+    // without a mask nothing behind the last row's own token is seen
+    const int t_hi = (pc.row0 + pc.rows - 1) / p.group;
+    const int seen = p.mask == nullptr ? min(s.len, s.ctx + t_hi + 1) : s.len;
+    pc.t0 = t0;
+    pc.t1 = min(t1, (seen + kKvTile - 1) / kKvTile);
+    return true;
+  }
+};
+
 __device__ __forceinline__ float kv_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -1,0 +1,724 @@
+// Attention over the quantised key/value cache for many query rows per kv head (trees of drafted tokens, prompt chunks) on
+// tcgen05, sm_100a.
+//
+// The mathematics is that of gl_kv_attend.cu.  With 128 rows a score costs more than a code, so the scales go into the codes
+// where that is safe: per tile of 128 tokens, with KS and VS powers of two set by the tile's largest scales,
+//   K'[p] = fp16(kq[p] ks[p] / KS),  V'[p] = fp16(vq[p] vs[p] / VS)          (one rounding of 2^-11 each; codes are exact)
+//   S = q K'^T,  P = 2^(a S + log2 VS - M + 7),  O += P V',  l += sum P / VS,  a = log2(e) c KS (times q's power of two)
+// and a score costs one multiply-add, one exponential, one maximum and one addition.  No number of such a tile is a subnormal
+// fp16 number as long as its scales lie within 2^12 of each other, so the choice of KS and VS changes no bit.  Tiles whose
+// scales lie further apart, and tiles with new tokens under a mask (a token that a row does not see must not round what it
+// sees), keep K' and V' at the codes and apply ks[p], log2 vs[p] and 1 / vs[p] to the scores, as the other kernel does.
+// M is a maximum of the exponents that lags: it is raised, and O and l are scaled, only when a row's new maximum is more than
+// 2^8 above it (P stays below 2^15 then, fp16's range, and keeps 31 binary orders below M).
+//
+// One persistent block per SM, 13 warps:
+//   warps 0-3, 4-7   two streams of 128 rows: scores out of TMEM, weights back into TMEM (over the scores), rescaling, output
+//   warps 8-11       codes from global memory (a tile ahead, in registers), conversion, swizzled shared memory (2 stages each)
+//   warp 12          one lane issues tcgen05.mma: S (operands in shared memory) and O (weights in TMEM, values MN-major)
+// While one stream's warps exponentiate, the tensor cores work on the other.  A unit with more than 128 live rows gives each
+// stream half of them, and both use every tile; with fewer, both streams hold the same rows and take every other tile, and
+// stream 1 hands its part to stream 0 at the end.
+#include "gl_kv_attend.cuh"
+#include "gl_tc_common.cuh"
+
+namespace {
+using namespace gltc;
+
+constexpr int kThreads = 16 * 32;             // 13 warps work; 16 fill the four warp groups that share out the registers
+constexpr int kMeta = 4;                       // tiles' scalars and masks: a tile's are read before the second tile after it is converted
+constexpr float kOff = 7.f, kRaise = 8.f;
+
+struct Meta {
+  float ks, vs_log2, vs_inv;
+  uint32_t apart;                              // the scales are in the arrays, not in the codes
+  uint32_t valid[4];
+  float col_ks[128], col_lv[128], col_rv[128];
+};
+
+template <int D> struct Lay {
+  static constexpr int HALF = 128 * 128;                           // 128 rows of 64 channels, 128-byte rows, 128-byte swizzle
+  static constexpr int TILE = HALF * (D / 64);
+  static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE, END = 6 * TILE;
+  static constexpr int SMEM = END + 1024;                          // base rounded up to 1024
+};
+
+struct Shared {
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full[2], p_full[2], q_full[2], o_full[2];
+  uint64_t x_full, x_empty, drain;
+  uint32_t tmem;
+  int abort, never;                            // set by a wait that gave up; never set
+  Meta meta[kMeta];
+  float2 xml[128];
+  KvPlaceScratch place;
+};
+
+// Descriptor of an MN-major operand: 64 channels per 128-byte row with 128-byte swizzle, 8-token groups 1024 bytes apart, blocks
+// of 64 channels 16 KB apart.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(16384 >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// finite positive maximum -> the power of two at or above it (1 if there is none); at least 2^-80
+__device__ __forceinline__ int pow2_above(uint32_t bits) {
+  if (bits == 0) return 0;
+  const int e = (int)(bits >> 23) - 127 + ((bits & 0x7fffffu) ? 1 : 0);
+  return min(max(e, -80), 126);
+}
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+
+// power of two that brings the largest code near the end of fp16's range
+template <int FMT> constexpr int kRoom = FMT == GL_KV_FP8 ? 7 : FMT == GL_KV_INT8 ? 8 : 12;
+constexpr int kSpread = 12;
+
+// scale ratio as two fp16 numbers (high, rest) of one value
+__device__ __forceinline__ uint32_t split_half(float r) {
+  const __half hi = __float2half_rn(r), lo = __float2half_rn(r - __half2float(hi));
+  return (uint32_t)__half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16;
+}
+__device__ __forceinline__ uint32_t scaled(uint32_t x, uint32_t hi2, uint32_t lo2) {
+  const __half2 v = *reinterpret_cast<__half2*>(&x), h = *reinterpret_cast<__half2*>(&hi2), l = *reinterpret_cast<__half2*>(&lo2);
+  const __half2 r = __hfma2(v, h, __hmul2(v, l));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// 32 lanes x 8 columns (x 4 for the store), complete on return: for the paths that are kept small rather than fast
+__device__ __forceinline__ void tmem_ld_8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st_4(uint32_t taddr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};\n\ttcgen05.wait::st.sync.aligned;"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+// a bounded wait of a whole warp: its lanes go on together, or give up together
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, nullptr, 0));
+}
+
+// ---- conversion warps ------------------------------------------------------------------------------------------------------
+template <int D, int FMT> struct Conv {
+  static constexpr int RB = FMT == GL_KV_INT4 ? D / 2 : D, CPT = RB / 16, N = 32 * RB / 16 / 32;    // N: 16-byte pieces per lane
+  static constexpr int TPI = 32 / CPT;                                                              // tokens per instruction
+
+  // 16 bytes of token row `tok` -> fp16, times the token's ratio, into the swizzled tile
+  static __device__ __forceinline__ void put(uint8_t* tile, int tok, int ch, const uint4& u, uint32_t ratio, uint32_t zero, bool zeros, bool nans) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    const uint32_t hi = __byte_perm(ratio, 0, 0x1010), lo = __byte_perm(ratio, 0, 0x3232);
+    constexpr int CH = FMT == GL_KV_INT4 ? 4 : 2;          // 16-byte chunks of fp16 that come out
+    uint32_t o[CH * 4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (FMT == GL_KV_INT4) {
+        uint32_t n[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) n[j] = kv_nibbles(w[i] >> (4 * j), zero);            // channels (j, j + 4)
+        o[4 * i] = __byte_perm(n[0], n[1], 0x5410);
+        o[4 * i + 1] = __byte_perm(n[2], n[3], 0x5410);
+        o[4 * i + 2] = __byte_perm(n[0], n[1], 0x7632);
+        o[4 * i + 3] = __byte_perm(n[2], n[3], 0x7632);
+      } else {
+        kv_bytes<FMT>(w[i], o[2 * i], o[2 * i + 1]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < CH * 4; ++i) {
+      o[i] = scaled(o[i], hi, lo);
+      if (zeros) o[i] = 0u;
+      if (nans) o[i] = 0x7fff7fffu;
+    }
+    const int c0 = ch * CH, half = c0 >> 3;
+    uint8_t* row = tile + half * Lay<D>::HALF + tok * 128;
+    // lanes of the two halves start with different chunks: their rows share the banks
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int j = CH == 2 && D == 128 ? i ^ half : i;
+      const int c = (c0 & 7) + j;
+      uint4 x = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+      if (CH == 2 && D == 128) {
+        x.x = half ? o[4 * (i ^ 1)] : o[4 * i];
+        x.y = half ? o[4 * (i ^ 1) + 1] : o[4 * i + 1];
+        x.z = half ? o[4 * (i ^ 1) + 2] : o[4 * i + 2];
+        x.w = half ? o[4 * (i ^ 1) + 3] : o[4 * i + 3];
+      }
+      *reinterpret_cast<uint4*>(row + ((c ^ (tok & 7)) << 4)) = x;
+    }
+  }
+};
+
+template <int D, int FMT>
+__device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh, uint8_t* base, KvWalk<kKvTcRows> walk) {
+  using C = Conv<D, FMT>;
+  const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - 8;        // this warp's tokens: 32 w .. 32 w + 31 of a tile
+  volatile int* abort = &sh.abort;
+  const KvBatch& kb = p.kb;
+
+  KvPiece pc;
+  bool have = walk.next(p, blockIdx.x, pc);
+  int tile = have ? pc.t0 : 0;
+  auto settle = [&]() {                                                   // to the next tile that exists
+    while (have && tile >= pc.t1) {
+      have = walk.next(p, blockIdx.x, pc);
+      tile = have ? pc.t0 : 0;
+    }
+  };
+  settle();
+
+  // One tile ahead: `slot` of the tile whose codes are loaded next (lane's token of each of its four 32-token parts).
+  int64_t slot[4];
+  bool draft_next = false;
+  auto locate = [&]() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int pos = tile * kKvTile + i * 32 + lane;
+      slot[i] = -1;
+      if (pos < pc.s.len) {
+        const int pi = p.page_shift >= 0 ? pos >> p.page_shift : pos / kb.page_size;
+        const int page = kb.page_table[(int64_t)walk.b * kb.pt_stride + pi];
+        if ((unsigned)page < (unsigned)kb.num_pages) slot[i] = ((int64_t)page * kb.hkv + pc.head) * kb.page_size + (pos - pi * kb.page_size);
+      }
+    }
+    draft_next = (tile + 1) * kKvTile > pc.s.ctx;
+  };
+  auto own = [&]() { return w == 0 ? slot[0] : w == 1 ? slot[1] : w == 2 ? slot[2] : slot[3]; };
+  auto load = [&](const uint8_t* codes, uint4 (&u)[C::N]) {
+    const int64_t mine = own();
+#pragma unroll
+    for (int i = 0; i < C::N; ++i) {
+      const int64_t s = __shfl_sync(0xffffffffu, mine, lane / C::CPT + i * C::TPI);
+      u[i] = make_uint4(0, 0, 0, 0);
+      if (s >= 0) u[i] = __ldg(reinterpret_cast<const uint4*>(codes + s * C::RB + (lane % C::CPT) * 16));
+    }
+  };
+  struct { float k[4], v[4]; uint32_t z, valid[4]; bool draft; } sc;
+  auto load_scales = [&]() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sc.k[i] = slot[i] >= 0 ? __ldg(p.k_scales + slot[i]) : 0.f;
+      sc.v[i] = slot[i] >= 0 ? __ldg(p.v_scales + slot[i]) : 0.f;
+      sc.valid[i] = __ballot_sync(0xffffffffu, slot[i] >= 0);
+    }
+    sc.draft = draft_next;
+    sc.z = 0;
+    if (FMT == GL_KV_INT4) {
+      const int64_t s = own();
+      if (s >= 0) sc.z = (uint32_t)__ldg(p.k_zeros + s) | (uint32_t)__ldg(p.v_zeros + s) << 8;
+    }
+  };
+
+  uint4 ku[C::N], vu[C::N];
+  bool live = have;
+  if (live) {
+    locate();
+    load(p.k_codes, ku);
+    load(p.v_codes, vu);
+    load_scales();
+    ++tile;
+    settle();
+    if (have) locate();
+  }
+  for (int n = 0; live; ++n) {
+    const int st = n & 1;
+    const uint32_t parity = ((n >> 1) & 1) ^ 1;
+    // the tile's powers of two, by every warp alike
+    uint32_t kt = 0, vt = 0, kl = 0x7f7fffffu, vl = 0x7f7fffffu;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t kbits = __float_as_uint(sc.k[i]), vbits = __float_as_uint(sc.v[i]);
+      if (kbits - 1u < 0x7f7fffffu) { kt = max(kt, kbits); kl = min(kl, kbits); }       // positive and finite
+      if (vbits - 1u < 0x7f7fffffu) { vt = max(vt, vbits); vl = min(vl, vbits); }
+    }
+    kt = __reduce_max_sync(0xffffffffu, kt);
+    vt = __reduce_max_sync(0xffffffffu, vt);
+    kl = __reduce_min_sync(0xffffffffu, kl);
+    vl = __reduce_min_sync(0xffffffffu, vl);
+    const bool apart = (sc.draft && p.mask != nullptr) || (int)(kt >> 23) - (int)(kl >> 23) >= kSpread || (int)(vt >> 23) - (int)(vl >> 23) >= kSpread;
+    const int ke = apart ? 0 : pow2_above(kt) - kRoom<FMT>, ve = apart ? 0 : pow2_above(vt) - kRoom<FMT>;
+    const float k_own = w == 0 ? sc.k[0] : w == 1 ? sc.k[1] : w == 2 ? sc.k[2] : sc.k[3], v_own = w == 0 ? sc.v[0] : w == 1 ? sc.v[1] : w == 2 ? sc.v[2] : sc.v[3];
+    const bool v_bad = !(fabsf(v_own) < INFINITY), v_none = v_own < 1e-30f;
+    const uint32_t kr = !(fabsf(k_own) < INFINITY) ? 0x00007fffu : apart ? 0x00003c00u : split_half(k_own * pow2(-ke));
+    const uint32_t vr = v_bad || (apart && v_none) ? 0u : apart ? 0x00003c00u : split_half(v_own * pow2(-ve));
+    // Values that are not numbers: as P V' they would reach every row, so V' is 0 there and K' is NaN, which the rows that
+    // see the token keep.  (Codes that are e4m3's NaN only matter where some rows do not see the token.)
+    uint32_t bad = __ballot_sync(0xffffffffu, v_bad);
+    if (FMT == GL_KV_FP8 && sc.draft) {
+#pragma unroll
+      for (int i = 0; i < C::N; ++i) {
+        const uint32_t m = 0x7f7f7f7fu, one = 0x01010101u;
+        const bool nan = (((((vu[i].x & m) + one) | ((vu[i].y & m) + one) | ((vu[i].z & m) + one) | ((vu[i].w & m) + one)) & 0x80808080u) != 0);
+        const uint32_t who = __ballot_sync(0xffffffffu, nan);
+#pragma unroll
+        for (int t = 0; t < C::TPI; ++t)
+          if ((who >> (t * C::CPT)) & ((1u << C::CPT) - 1u)) bad |= 1u << (t + i * C::TPI);
+      }
+    }
+    const uint32_t zk = 0x6400u + (sc.z & 255u), zv = 0x6400u + (sc.z >> 8);
+
+    if (n >= 2 && !warp_wait(&sh.k_empty[st], parity, abort)) return;
+    if (lane == 0 && w == 0) {
+      Meta& m = sh.meta[n % kMeta];
+      m.apart = apart;
+      m.ks = pow2(ke);
+      m.vs_log2 = (float)ve;
+      m.vs_inv = pow2(-ve);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m.valid[i] = sc.valid[i];
+    }
+    if (apart) {
+      Meta& m = sh.meta[n % kMeta];
+      const float v = v_none ? 1e-30f : v_own;
+      m.col_ks[w * 32 + lane] = k_own;
+      m.col_lv[w * 32 + lane] = __log2f(v);
+      m.col_rv[w * 32 + lane] = __frcp_rn(v);
+    }
+    uint8_t* kt_s = base + Lay<D>::K + st * Lay<D>::TILE;
+    uint8_t* vt_s = base + Lay<D>::V + st * Lay<D>::TILE;
+#pragma unroll
+    for (int i = 0; i < C::N; ++i) {
+      const int t = lane / C::CPT + i * C::TPI;
+      const uint32_t r = __shfl_sync(0xffffffffu, kr, t);
+      uint32_t z = 0;
+      if (FMT == GL_KV_INT4) { z = __shfl_sync(0xffffffffu, zk, t); z |= z << 16; }
+      C::put(kt_s, w * 32 + t, lane % C::CPT, ku[i], r, z, false, (bad >> t) & 1u);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.k_full[st]);
+    const bool more = have;
+    if (more) {
+      load(p.k_codes, ku);
+      load_scales();
+    }
+    if (n >= 2 && !warp_wait(&sh.v_empty[st], parity, abort)) return;
+#pragma unroll
+    for (int i = 0; i < C::N; ++i) {
+      const int t = lane / C::CPT + i * C::TPI;
+      const uint32_t r = __shfl_sync(0xffffffffu, vr, t);
+      uint32_t z = 0;
+      if (FMT == GL_KV_INT4) { z = __shfl_sync(0xffffffffu, zv, t); z |= z << 16; }
+      C::put(vt_s, w * 32 + t, lane % C::CPT, vu[i], r, z, (bad >> t) & 1u, false);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.v_full[st]);
+    if (more) {
+      load(p.v_codes, vu);
+      ++tile;
+      settle();
+      if (have) locate();
+    }
+    live = more;
+  }
+}
+
+// ---- the MMA lane ------------------------------------------------------------------------------------------------------------
+template <int D>
+__device__ __forceinline__ void mma_role(const KvAttendParams& p, Shared& sh, uint32_t base, KvWalk<kKvTcRows> walk, uint32_t idesc_s, uint32_t idesc_o) {
+  volatile int* abort = &sh.abort;
+  const uint32_t tm = sh.tmem;
+  KvPiece pc;
+  int n0 = 0;                                  // tiles of earlier pieces
+  uint32_t q_phase = 0, p_phase[2] = {0, 0};
+  while (walk.next(p, blockIdx.x, pc)) {
+    const int n = pc.t1 - pc.t0;
+    if (n <= 0) continue;
+    const bool both = pc.rows > 128;
+    const int events = both ? 2 * n : n;
+    auto scores = [&](int e) -> bool {
+      const int s = e & 1, j = n0 + (both ? e >> 1 : e), st = j & 1;
+      if ((!both || s == 0) && !mbar_wait_spin(&sh.k_full[st], (j >> 1) & 1, abort, nullptr, 0)) return false;
+      tc_fence_after();
+      const uint32_t q = base + Lay<D>::Q + s * Lay<D>::TILE, k = base + Lay<D>::K + st * Lay<D>::TILE;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t off = (kk >> 2) * Lay<D>::HALF + (kk & 3) * 32;
+        mma_ss<KIND_F16>(tm + s * 128, smem_desc_sw128(q + off), smem_desc_sw128(k + off), idesc_s, kk > 0);
+      }
+      tc_commit(&sh.s_full[s]);
+      if (!both || s == 1) tc_commit(&sh.k_empty[st]);
+      return true;
+    };
+    for (int s = 0; s < 2; ++s)
+      if (!mbar_wait_spin(&sh.q_full[s], q_phase, abort, nullptr, 0)) return;
+    q_phase ^= 1;
+    tc_fence_after();
+    for (int e = 0; e < 2 && e < events; ++e)
+      if (!scores(e)) return;
+    for (int e = 0; e < events; ++e) {
+      const int s = e & 1, i = both ? e >> 1 : e, j = n0 + i, st = j & 1;
+      if ((!both || s == 0) && !mbar_wait_spin(&sh.v_full[st], (j >> 1) & 1, abort, nullptr, 0)) return;
+      if (!mbar_wait_spin(&sh.p_full[s], p_phase[s], abort, nullptr, 0)) return;
+      p_phase[s] ^= 1;
+      tc_fence_after();
+      const uint32_t v = base + Lay<D>::V + st * Lay<D>::TILE;
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk)
+        mma_ts_f16(tm + 256 + s * D, tm + s * 128 + kk * 8, desc_mn(v + kk * 2048), idesc_o, e >= 2 || kk > 0);
+      if (!both || s == 1) tc_commit(&sh.v_empty[st]);
+      if (e + 2 >= events) tc_commit(&sh.o_full[s]);
+      else if (!scores(e + 2)) return;
+    }
+    n0 += n;
+  }
+}
+
+// ---- the two streams ---------------------------------------------------------------------------------------------------------
+template <int D, typename T>
+__device__ __forceinline__ void stream_role(const KvAttendParams& p, Shared& sh, uint8_t* base, KvWalk<kKvTcRows> walk) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, s = warp >> 2, row = threadIdx.x & 127;
+  volatile int* abort = &sh.abort;
+  const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+  const uint32_t ts = sh.tmem + lanes + s * 128, to = sh.tmem + lanes + 256 + s * D;
+  KvPiece pc;
+  int n0 = 0, merges = 0;
+  uint32_t s_phase = 0, o_phase = 0;
+  bool ok = true;
+  while (walk.next(p, blockIdx.x, pc)) {
+    const int n = pc.t1 - pc.t0 > 0 ? pc.t1 - pc.t0 : 0;
+    const bool both = pc.rows > 128;
+    const int r = both ? s * 128 + row : row;                    // row of the unit
+    const bool live = r < pc.rows;
+    const int rr = pc.row0 + (live ? r : 0), tok = rr / p.group, head = pc.head * p.group + (rr - tok * p.group);
+    float m_used = -INFINITY, l = 0.f;
+    const int mine = both ? n : s == 0 ? (n + 1) / 2 : n / 2;
+    if (n > 0 && ok) {
+      // ---- queries: fp16 by a power of two, into this stream's swizzled tile
+      if (merges > 0) ok = warp_wait(&sh.x_empty, (merges - 1) & 1, abort);
+      const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)(pc.s.first + tok) * p.q_sn + (int64_t)head * p.q_sh;
+      float factor = 1.f, inv = 1.f;
+      if constexpr (!IsHalf<T>::value) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const uint4 u = live ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0, 0, 0, 0);
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top = max(top, max(w[j] & 0x7fffu, (w[j] >> 16) & 0x7fffu));
+        }
+        const int ex = min(max((int)(top >> 7), 1), 253);
+        inv = __int_as_float((254 - ex) << 23);
+        factor = __int_as_float(ex << 23);
+      }
+      // the sign of the scale goes into the queries: maxima are taken of the scores themselves
+      const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+      const float qs = fabsf(p.scale_log2) * factor;
+      uint8_t* qt = base + Lay<D>::Q + s * Lay<D>::TILE + row * 128;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        uint4 u = live ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0, 0, 0, 0);
+        uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (!IsHalf<T>::value) {
+            const __half2 h = __floats2half2_rn(__uint_as_float(w[j] << 16) * inv, __uint_as_float(w[j] & 0xffff0000u) * inv);
+            w[j] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+          w[j] ^= flip;
+        }
+        *reinterpret_cast<uint4*>(qt + (i >> 3) * Lay<D>::HALF + (((i & 7) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.q_full[s]);
+
+      const int t_lo = (pc.row0 + (both ? s * 128 : 0)) / p.group;      // the stream's first row's token
+      for (int i = 0; i < mine && ok; ++i) {
+        const int j = both ? i : 2 * i + s;
+        const Meta& meta = sh.meta[(n0 + j) % kMeta];
+        ok = warp_wait(&sh.s_full[s], s_phase, abort);
+        if (!ok) break;
+        s_phase ^= 1;
+        tc_fence_after();
+        const int tile0 = (pc.t0 + j) * kKvTile;
+        const uint4 vld = make_uint4(meta.valid[0], meta.valid[1], meta.valid[2], meta.valid[3]);
+        const bool full = meta.apart == 0 && (vld.x & vld.y & vld.z & vld.w) == 0xffffffffu && tile0 + kKvTile <= pc.s.ctx + (p.mask == nullptr ? t_lo + 1 : 0);
+        const float a = qs * meta.ks, lv = meta.vs_log2;
+        uint32_t seen[4] = {vld.x, vld.y, vld.z, vld.w};
+        if (!full) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int at = tile0 + 32 * w - pc.s.ctx;                  // the word's first token: which new token
+            if (at + 32 <= 0) continue;
+            if (p.mask == nullptr) {
+              const int k = tok + 1 - at;
+              seen[w] &= k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1u;
+            } else {
+              const uint8_t* mk = p.mask + (int64_t)(pc.s.first + tok) * p.mask_stride;
+              for (int k = max(0, -at); k < 32; ++k)
+                if ((seen[w] >> k) & 1u)
+                  if (at + k >= p.mask_cols || mk[at + k] == 0) seen[w] &= ~(1u << k);
+            }
+          }
+        }
+        const bool apart = meta.apart != 0;
+        auto exponent = [&](float sc, int col) { return apart ? fmaf(sc * meta.col_ks[col], qs, meta.col_lv[col]) : fmaf(sc, a, lv); };
+        // ---- the tile's maximum.  (The paths for tiles that are not full are rolled up: unrolled, the kernel outgrew the
+        // instruction cache and ran at a fifth of its speed.)
+        float top = -INFINITY;
+        uint32_t x[2][32];
+        if (full) {
+#pragma unroll 1
+          for (int h = 0; h < 128; h += 64) {
+            tmem_ld_32x32_issue(ts + h, x[0]);
+            tmem_ld_32x32_issue(ts + h + 32, x[1]);
+            tmem_ld_wait();
+            tmem_ld_fence(x[0]);
+            tmem_ld_fence(x[1]);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) top = fmaxf(top, fmaxf(__uint_as_float(x[0][k]), __uint_as_float(x[1][k])));
+          }
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 8) {
+            uint32_t y[8];
+            tmem_ld_8(ts + c, y);
+            const uint32_t sw = (c < 64 ? (c < 32 ? seen[0] : seen[1]) : (c < 96 ? seen[2] : seen[3])) >> (c & 31);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) top = (sw >> k) & 1u ? fmaxf(top, exponent(__uint_as_float(y[k]), c + k)) : top;
+          }
+        }
+        const float t_top = full ? fmaf(top, a, lv) : top;
+        const bool raise = t_top > m_used + kRaise || (m_used == -INFINITY && t_top != -INFINITY);
+        if (__any_sync(0xffffffffu, raise)) {
+          const float m_new = fmaxf(m_used, t_top), f = m_used == m_new ? 1.f : kv_exp2(m_used - m_new);
+          l *= f;
+          m_used = m_new;
+          if (i > 0) {                                                // (s_full: the products before this tile's scores are done)
+#pragma unroll 1
+            for (int d = 0; d < D; d += 32) {
+              tmem_ld_32x32(to + d, x[0]);
+              tmem_ld_fence(x[0]);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) x[0][k] = __float_as_uint(__uint_as_float(x[0][k]) * f);
+              tmem_st_32x32(to + d, x[0]);
+            }
+          }
+        }
+        // ---- weights, over the scores
+        const float to_p = m_used == -INFINITY ? 0.f : kOff - m_used, sub = lv + to_p, inv_vs = meta.vs_inv;
+        float sum = 0.f;
+        if (full) {
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            tmem_ld_32x32_issue(ts + h * 64, x[0]);
+            tmem_ld_32x32_issue(ts + h * 64 + 32, x[1]);
+            tmem_ld_wait();
+            tmem_ld_fence(x[0]);
+            tmem_ld_fence(x[1]);
+            uint32_t pk[32];
+            float s1 = 0.f;
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+              for (int k = 0; k < 32; k += 2) {
+                const float e0 = kv_exp2(fmaf(__uint_as_float(x[q][k]), a, sub)), e1 = kv_exp2(fmaf(__uint_as_float(x[q][k + 1]), a, sub));
+                sum += e0;
+                s1 += e1;
+                const __half2 hh = __floats2half2_rn(e0, e1);
+                pk[q * 16 + (k >> 1)] = *reinterpret_cast<const uint32_t*>(&hh);
+              }
+            sum += s1;
+            tmem_st_32x32(ts + h * 32, pk);
+          }
+          sum *= inv_vs;
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 8) {
+            uint32_t y[8], pk[4];
+            tmem_ld_8(ts + c, y);
+            const uint32_t sw = (c < 64 ? (c < 32 ? seen[0] : seen[1]) : (c < 96 ? seen[2] : seen[3])) >> (c & 31);
+            float e[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              e[k] = (sw >> k) & 1u ? kv_exp2(exponent(__uint_as_float(y[k]), c + k) + to_p) : 0.f;
+              sum += (sw >> k) & 1u ? e[k] * (apart ? meta.col_rv[c + k] : inv_vs) : 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const __half2 hh = __floats2half2_rn(e[2 * k], e[2 * k + 1]);
+              pk[k] = *reinterpret_cast<const uint32_t*>(&hh);
+            }
+            tmem_st_4(ts + c / 2, pk);
+          }
+        }
+        l += sum;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.p_full[s]);
+      }
+      if (mine > 0 && ok) {
+        ok = warp_wait(&sh.o_full[s], o_phase, abort);
+        o_phase ^= 1;
+        tc_fence_after();
+      }
+    }
+
+    // ---- the result of the unit, or of its part
+    const bool merge = !both && n > 1;
+    float m1 = -INFINITY, l1 = 0.f;
+    const float4* other = reinterpret_cast<const float4*>(base + Lay<D>::Q) + row;      // [D / 4][128]: the streams' queries are done with
+    if (merge && s == 1) {
+      uint32_t x[32];
+      if (ok) {
+#pragma unroll 1
+        for (int d = 0; d < D; d += 32) {
+          tmem_ld_32x32(to + d, x);
+          tmem_ld_fence(x);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) const_cast<float4*>(other)[(d / 4 + k) * 128] = make_float4(__uint_as_float(x[4 * k]), __uint_as_float(x[4 * k + 1]), __uint_as_float(x[4 * k + 2]), __uint_as_float(x[4 * k + 3]));
+        }
+        sh.xml[row] = make_float2(m_used, l);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.x_full);
+      }
+    }
+    if (both || s == 0) {
+      if (merge && ok) {
+        ok = warp_wait(&sh.x_full, merges & 1, abort);
+        const float2 ml = sh.xml[row];
+        m1 = ml.x;
+        l1 = ml.y;
+      }
+      const float top = fmaxf(m_used, m1);
+      const float f0 = m_used == -INFINITY ? (l == 0.f ? 0.f : 1.f) : kv_exp2(m_used - top), f1 = m1 == -INFINITY ? (l1 == 0.f ? 0.f : 1.f) : kv_exp2(m1 - top);
+      float lt = l * f0 + l1 * f1;
+      if (!ok) lt = __int_as_float(0x7fc00000);                     // a wait ran out: the rows say so
+      const float rcp = lt == 0.f ? 0.f : 1.f / lt;
+      uint32_t x[32];
+      T* dst = reinterpret_cast<T*>(p.out) + ((int64_t)(pc.s.first + tok) * p.hq + head) * D;
+      const int64_t pr = (int64_t)pc.slot * kKvTcRows + r;
+#pragma unroll 1
+      for (int d = 0; d < D; d += 32) {
+        if (mine > 0) {
+          tmem_ld_32x32(to + d, x);
+          tmem_ld_fence(x);
+        }
+        float v[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] = mine > 0 ? __uint_as_float(x[k]) * f0 : 0.f;
+        if (merge) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float4 y = other[(d / 4 + k) * 128];
+            v[4 * k] = fmaf(y.x, f1, v[4 * k]);
+            v[4 * k + 1] = fmaf(y.y, f1, v[4 * k + 1]);
+            v[4 * k + 2] = fmaf(y.z, f1, v[4 * k + 2]);
+            v[4 * k + 3] = fmaf(y.w, f1, v[4 * k + 3]);
+          }
+        }
+        if (live) {
+          if (pc.whole) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t o[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float a0 = lt == 0.f ? 0.f : v[8 * k + 2 * j] * rcp, a1 = lt == 0.f ? 0.f : v[8 * k + 2 * j + 1] * rcp;
+                if constexpr (IsHalf<T>::value) {
+                  const __half2 h = __floats2half2_rn(a0, a1);
+                  o[j] = *reinterpret_cast<const uint32_t*>(&h);
+                } else {
+                  const __nv_bfloat162 h = __floats2bfloat162_rn(a0, a1);
+                  o[j] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+              }
+              *reinterpret_cast<uint4*>(dst + d + 8 * k) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) *reinterpret_cast<float4*>(p.part_o + pr * D + d + 4 * k) = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+          }
+        }
+      }
+      if (live && !pc.whole) p.part_ml[pr] = make_float2(top, lt);
+      tc_fence_before();
+      if (merge && s == 0) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.x_empty);
+      }
+    }
+    if (merge) ++merges;
+    n0 += n;
+  }
+}
+
+template <int D, int FMT, typename T>
+__global__ void __launch_bounds__(kThreads, 1) kv_attend_tc_kernel(const KvAttendParams p, uint32_t idesc_s, uint32_t idesc_o) {
+  extern __shared__ uint8_t raw[];
+  __shared__ Shared sh;
+  uint8_t* base = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.k_full[i], 4);
+      mbar_init(&sh.v_full[i], 4);
+      mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.v_empty[i], 1);
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.q_full[i], 4);
+      mbar_init(&sh.o_full[i], 1);
+    }
+    mbar_init(&sh.x_full, 4);
+    mbar_init(&sh.x_empty, 4);
+    mbar_init(&sh.drain, 1);
+    sh.abort = sh.never = 0;
+    fence_barrier_init();
+  }
+  if (warp == 12) tmem_alloc(&sh.tmem, 512);
+  gl_launch_dependents();
+  gl_grid_dependency_wait();
+  KvWalk<kKvTcRows> walk;
+  walk.start(p, kv_place_of_block<kKvTcRows, kThreads>(p, blockIdx.x, sh.place), blockIdx.x);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+
+  // Every wait is bounded; one that gives up ends all roles, and the rows that it leaves unfinished become NaN.
+  // Registers: 512 threads are launched with 128 each; 3 x 152 + 56 = 512 are what they are given again.
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+    stream_role<D, T>(p, sh, base, walk);
+  } else if (warp < 12) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+    convert_role<D, FMT>(p, sh, base, walk);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (threadIdx.x == 12 * 32) {
+      mma_role<D>(p, sh, smem_u32(base), walk, idesc_s, idesc_o);
+      // nothing of this block's is in flight when the TMEM goes back
+      tc_commit(&sh.drain);
+      mbar_wait(&sh.drain, 0, &sh.never, nullptr, 0);
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12) tmem_dealloc(sh.tmem, 512);
+}
+
+template <int D, int FMT, typename T>
+int launch(const KvAttendParams& p, cudaStream_t st) {
+  if (int rc = kv_allow_smem((const void*)kv_attend_tc_kernel<D, FMT, T>, Lay<D>::SMEM)) return rc;
+  const uint32_t idesc_s = gl_idesc(1, 0, 0, 128, kKvTile), idesc_o = gl_idesc(1, 0, 0, 128, D) | (1u << 16);     // bit 16: B is MN-major
+  GL_CUDA_CHECK(gl_launch_pdl(kv_attend_tc_kernel<D, FMT, T>, dim3((unsigned)p.blocks), dim3(kThreads), Lay<D>::SMEM, st, p, idesc_s, idesc_o));
+  return GL_OK;
+}
+template <int D, typename T>
+int launch_fmt(const KvAttendParams& p, int fmt, cudaStream_t st) {
+  switch (fmt) {
+    case GL_KV_FP8: return launch<D, GL_KV_FP8, T>(p, st);
+    case GL_KV_INT8: return launch<D, GL_KV_INT8, T>(p, st);
+    default: return launch<D, GL_KV_INT4, T>(p, st);
+  }
+}
+
+}  // namespace
+
+int gl_kv_attend_tc_launch(const KvAttendParams& p, int head_dim, int format, int x_dtype, cudaStream_t st) {
+  if (head_dim == 128) return x_dtype == GL_BF16 ? launch_fmt<128, __nv_bfloat16>(p, format, st) : launch_fmt<128, __half>(p, format, st);
+  return x_dtype == GL_BF16 ? launch_fmt<64, __nv_bfloat16>(p, format, st) : launch_fmt<64, __half>(p, format, st);
+}

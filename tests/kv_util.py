@@ -52,6 +52,15 @@ def scales64(cache, which, page_table, b, count):
     return torch.stack(rows).double() if rows else torch.empty((0, cache.n_kv_heads), dtype=torch.float64, device=s.device)
 
 
+def score_slack64(q, k, sees, scale):
+    """[t, h]: what rounding the keys to fp16 (unit 2^-11, a product's error uniform in it: 2^-11 / sqrt 3 of the product) may add
+    to a score: 6 sigma of a row's worst seen token."""
+    g = q.shape[1] // k.shape[1]
+    k = torch.where(sees.any(0)[:, None, None], k, 0.0)
+    out = [((q[:, h].double() ** 2) @ (k[:, h // g] ** 2).T * sees).amax(1).sqrt() for h in range(q.shape[1])]
+    return torch.stack(out, 1) * abs(scale) * 2.0 ** -11 * 6 / math.sqrt(3)
+
+
 def attend64(q, k, v, sees, scale, v_scales=None):
     """q [t, h, d], k / v [l, hkv, d] fp64, sees bool [t, l] -> (result [t, h, d], sum of p |v| [t, h, d]); zeros where a row sees
     nothing.  Tokens that no row may see can hold anything.

@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from tests.kv_util import attend64, held64, make_cache, norm64, rotate64, scales64
+from tests.kv_util import attend64, held64, make_cache, norm64, rotate64, scales64, score_slack64
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -163,12 +163,17 @@ def _tree(seed, new, width):
     return torch.cat(rows).to(DEV)
 
 
-def _check_attend(cache, table, ctx, new, q, mask, out, scale=None):
+def _check_attend(cache, table, ctx, new, q, mask, out, scale=None, rounds_codes=False):
     """Against fp64.  Per element: half a step of the output's type, and of sum p |v|: 2^-11 for the weights' rounding to fp16,
     2^-12 for the exponents (scores of up to about 40 with fp32 sums over 128 products: 40 * 128 * 2^-24 * log2 e < 2^-11
     at the very worst, and sums do not line up), doubled for the denominator; what the smallest weights lose in fp16 is
     counted by attend64 (first run without it: a weight of 2^-34 beside one of 1, on a channel where the large one's code is
-    0, was off by 0.8 %; its fp16 number 2^-19 has a step of 2^-24)."""
+    0, was off by 0.8 %; its fp16 number 2^-19 has a step of 2^-24).
+
+    rounds_codes: the kernel for many rows rounds scaled values and keys to fp16: 2^-11 of sum p |v| for the values, and for
+    the keys twice (numerator, denominator) what score_slack64 says; its smallest weights have 2^-31 of the largest as their
+    last normal order, 2^8 times the other kernel's floor."""
+    rounds_codes = rounds_codes or max(new) * (q.shape[1] // cache.n_kv_heads) > 32
     at = 0
     for b, (c, t) in enumerate(zip(ctx, new)):
         if t == 0:
@@ -184,6 +189,10 @@ def _check_attend(cache, table, ctx, new, q, mask, out, scale=None):
         want, size = attend64(q[at:at + t], k, v, sees, 1 / math.sqrt(cache.head_dim) if scale is None else scale,
                               scales64(cache, "v", table, b, cap))
         tol = torch.finfo(q.dtype).eps / 2 * want.abs() + 2.0 ** -9.5 * size + (2.0 ** -25 if q.dtype == torch.float16 else 0)
+        if rounds_codes:
+            plain = attend64(q[at:at + t], k, v, sees, 1 / math.sqrt(cache.head_dim) if scale is None else scale)[1]
+            slack = score_slack64(q[at:at + t], k, sees, 1 / math.sqrt(cache.head_dim) if scale is None else scale)
+            tol = tol + 2.0 ** -11 * plain + 2 * slack[..., None] * plain + (2.0 ** 8 - 1) * 2.0 ** -9.5 * (size - plain)
         err = (out[at:at + t].double() - want).abs()
         assert bool((err <= tol).all()), (b, float((err / tol.clamp(min=1e-30)).max()))
         at += t
@@ -211,17 +220,20 @@ def test_attend_matches_the_formula(lib, fmt, d, dtype, shape):
     q = _randn(shape, sum(new), hq, d, dtype=dtype, scale=1.5)
     off = _i32([0] + torch.tensor(new).cumsum(0).tolist())
     batch = KVBatch(table, _i32(ctx), off, max_len=max(c + t for c, t in zip(ctx, new)), max_new=max(new))
-    _check_attend(cache, table, ctx, new, q, None, cache.attend(q, batch))
+    for kernel in (0, 1, 2):
+        _check_attend(cache, table, ctx, new, q, None, cache.attend(q, batch, kernel_override=kernel), rounds_codes=kernel == 2)
     tree = _tree(shape, new, max(new))
     _check_attend(cache, table, ctx, new, q, tree, cache.attend(q, batch, mask=tree))
     # any mask: rows that see none of the new tokens (nothing at all where nothing is cached), tokens that nobody sees
     g = torch.Generator(device=DEV).manual_seed(shape)
     some = torch.rand(tree.shape, generator=g, device=DEV) < 0.3
     some[::3] = False
-    _check_attend(cache, table, ctx, new, q, some, cache.attend(q, batch, mask=some))
-    # bounds that say nothing or too little change no result beyond the order of sums
+    for kernel in (0, 1, 2):
+        _check_attend(cache, table, ctx, new, q, some, cache.attend(q, batch, mask=some, kernel_override=kernel), rounds_codes=kernel == 2)
+    # bounds that say nothing (all rows might be one sequence's: the kernel for many rows) or too little change no result
+    # beyond that kernel's roundings and the order of sums
     for kw in ({}, {"max_len": 1, "max_new": 1}):
-        _check_attend(cache, table, ctx, new, q, tree, cache.attend(q, KVBatch(table, _i32(ctx), off, **kw), mask=tree.to(torch.uint8)))
+        _check_attend(cache, table, ctx, new, q, tree, cache.attend(q, KVBatch(table, _i32(ctx), off, **kw), mask=tree.to(torch.uint8)), rounds_codes=True)
 
 
 @pytest.mark.parametrize("fmt", FMTS)

@@ -46,9 +46,9 @@ def test_unsupported_and_call_specific(lib):
     for bad in ({"rot_dim": 24}, {"rot_dim": 144}, {"rot_dim": 64}, {"k": None}, {"q_stride_n": 4}, {"v": (1 << 20) + 2},
                 {"q_norm": 1 << 20, "norm_dtype": 4}, {"n_q_heads": 0}):
         assert lib.gl_kv_write(ctypes.byref(_args(**bad)), None) == _lib.GL_E_INVALID, bad
-    for bad in ({"n_q_heads": 3}, {"n_q_heads": 0}, {"q": None}, {"q_stride_h": 12}, {"mask": 1 << 20, "mask_cols": -1}):
+    for bad in ({"n_q_heads": 3}, {"n_q_heads": 0}, {"q": None}, {"q_stride_h": 12}, {"mask": 1 << 20, "mask_cols": -1}, {"kernel_override": 3}):
         assert lib.gl_kv_attend(ctypes.byref(_args(**bad)), None) == _lib.GL_E_INVALID, bad
-    assert lib.gl_kv_attend(ctypes.byref(_args(batch=1 << 17, n_tokens=1 << 17)), None) == _lib.GL_E_UNSUPPORTED
+    assert lib.gl_kv_attend(ctypes.byref(_args(n_q_heads=1 << 16, n_kv_heads=1, n_tokens=1 << 16)), None) == _lib.GL_E_UNSUPPORTED
     assert lib.gl_kv_attend(ctypes.byref(_args(max_pages=1 << 28)), None) == _lib.GL_E_UNSUPPORTED
     long = _args(max_pages=1 << 12, max_len=1 << 16)
     need = lib.gl_kv_attend_workspace_bytes(ctypes.byref(long))
