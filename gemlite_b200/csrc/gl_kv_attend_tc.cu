@@ -2,20 +2,21 @@
 // tcgen05, sm_100a.
 //
 // The mathematics is that of gl_kv_attend.cu.  With 128 rows a score costs more than a code, so the scales go into the codes
-// where that is safe: per tile of 128 tokens, with KS and VS powers of two set by the tile's largest scales,
+// where that is safe: per 32 tokens, with KS and VS powers of two set by their largest scales,
 //   K'[p] = fp16(kq[p] ks[p] / KS),  V'[p] = fp16(vq[p] vs[p] / VS)          (one rounding of 2^-11 each; codes are exact)
 //   S = q K'^T,  P = 2^(a S + log2 VS - M + 7),  O += P V',  l += sum P / VS,  a = log2(e) c KS (times q's power of two)
-// and a score costs one multiply-add, one exponential, one maximum and one addition.  No number of such a tile is a subnormal
-// fp16 number as long as its scales lie within 2^12 of each other, so the choice of KS and VS changes no bit.  Tiles whose
-// scales lie further apart, and tiles with new tokens under a mask (a token that a row does not see must not round what it
-// sees), keep K' and V' at the codes and apply ks[p], log2 vs[p] and 1 / vs[p] to the scores, as the other kernel does.
+// and a score costs one multiply-add, one exponential, one maximum and one addition.  None of these numbers is a subnormal
+// fp16 number as long as the scales lie within 2^12 of each other, so the choice of KS and VS changes no bit.  Where scales
+// lie further apart, and where tiles hold new tokens under a mask (a token that a row does not see must not round what it
+// sees), K' or V' stay the codes, and ks[p], or log2 vs[p] and 1 / vs[p], go to the scores, as in the other kernel.
 // M is a maximum of the exponents that lags: it is raised, and O and l are scaled, only when a row's new maximum is more than
 // 2^8 above it (P stays below 2^15 then, fp16's range, and keeps 31 binary orders below M).
 //
-// One persistent block per SM, 13 warps:
-//   warps 0-3, 4-7   two streams of 128 rows: scores out of TMEM, weights back into TMEM (over the scores), rescaling, output
-//   warps 8-11       codes from global memory (a tile ahead, in registers), conversion, swizzled shared memory (2 stages each)
-//   warp 12          one lane issues tcgen05.mma: S (operands in shared memory) and O (weights in TMEM, values MN-major)
+// One persistent block per SM, 17 working warps:
+//   warps 0-3, 4-7    two streams of 128 rows: scores out of TMEM, weights back into TMEM (over the scores), rescaling, output
+//   warps 8-11, 12-15 keys and values: codes from global memory (a tile ahead, in registers), conversion, swizzled shared
+//                     memory (2 stages each); a warp takes 32 tokens of every tile
+//   warp 16           one lane issues tcgen05.mma: S (operands in shared memory) and O (weights in TMEM, values MN-major)
 // While one stream's warps exponentiate, the tensor cores work on the other.  A unit with more than 128 live rows gives each
 // stream half of them, and both use every tile; with fewer, both streams hold the same rows and take every other tile, and
 // stream 1 hands its part to stream 0 at the end.
@@ -25,13 +26,13 @@
 namespace {
 using namespace gltc;
 
-constexpr int kThreads = 16 * 32;             // 13 warps work; 16 fill the four warp groups that share out the registers
+constexpr int kThreads = 20 * 32;             // 17 warps work; 20 fill the five warp groups that share out the registers
 constexpr int kMeta = 4;                       // tiles' scalars and masks: a tile's are read before the second tile after it is converted
 constexpr float kOff = 7.f, kRaise = 8.f;
 
-struct Meta {
-  float ks, vs_log2, vs_inv;
-  uint32_t apart;                              // the scales are in the arrays, not in the codes
+struct alignas(16) Meta {                      // per 32 tokens; read as 16-byte vectors
+  float ks[4], vs_log2[4], vs_inv[4];
+  uint32_t k_apart[4], v_apart[4];             // the scales are in the arrays, not in the codes
   uint32_t valid[4];
   float col_ks[128], col_lv[128], col_rv[128];
 };
@@ -92,6 +93,12 @@ __device__ __forceinline__ void tmem_st_4(uint32_t taddr, const uint32_t (&r)[4]
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};\n\ttcgen05.wait::st.sync.aligned;"
                ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
 }
+__device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&r)[16]) {      // tmem_st_wait() must follow
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+                 "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // a bounded wait of a whole warp: its lanes go on together, or give up together
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, nullptr, 0));
@@ -101,9 +108,13 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 template <int D, int FMT> struct Conv {
   static constexpr int RB = FMT == GL_KV_INT4 ? D / 2 : D, CPT = RB / 16, N = 32 * RB / 16 / 32;    // N: 16-byte pieces per lane
   static constexpr int TPI = 32 / CPT;                                                              // tokens per instruction
+  // token (of TPI) and 16-byte piece of its row that a lane takes: eight lanes that store together hold two tokens and, of
+  // 128-byte rows, one half each, which the swizzle spreads over all banks
+  static __device__ __forceinline__ int token(int lane) { return CPT == 8 ? (lane >> 4) * 2 + ((lane >> 2) & 1) : lane / CPT; }
+  static __device__ __forceinline__ int piece(int lane) { return CPT == 8 ? ((lane >> 3) & 1) * 4 + (lane & 3) : lane % CPT; }
 
   // 16 bytes of token row `tok` -> fp16, times the token's ratio, into the swizzled tile
-  static __device__ __forceinline__ void put(uint8_t* tile, int tok, int ch, const uint4& u, uint32_t ratio, uint32_t zero, bool zeros, bool nans) {
+  static __device__ __forceinline__ void put(uint8_t* tile, int tok, int ch, const uint4& u, uint32_t ratio, uint32_t zero) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
     const uint32_t hi = __byte_perm(ratio, 0, 0x1010), lo = __byte_perm(ratio, 0, 0x3232);
     constexpr int CH = FMT == GL_KV_INT4 ? 4 : 2;          // 16-byte chunks of fp16 that come out
@@ -122,193 +133,148 @@ template <int D, int FMT> struct Conv {
         kv_bytes<FMT>(w[i], o[2 * i], o[2 * i + 1]);
       }
     }
+    const int c0 = ch * CH;
+    uint8_t* row = tile + (c0 >> 3) * Lay<D>::HALF + tok * 128;
 #pragma unroll
-    for (int i = 0; i < CH * 4; ++i) {
-      o[i] = scaled(o[i], hi, lo);
-      if (zeros) o[i] = 0u;
-      if (nans) o[i] = 0x7fff7fffu;
-    }
-    const int c0 = ch * CH, half = c0 >> 3;
-    uint8_t* row = tile + half * Lay<D>::HALF + tok * 128;
-    // lanes of the two halves start with different chunks: their rows share the banks
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int j = CH == 2 && D == 128 ? i ^ half : i;
-      const int c = (c0 & 7) + j;
-      uint4 x = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-      if (CH == 2 && D == 128) {
-        x.x = half ? o[4 * (i ^ 1)] : o[4 * i];
-        x.y = half ? o[4 * (i ^ 1) + 1] : o[4 * i + 1];
-        x.z = half ? o[4 * (i ^ 1) + 2] : o[4 * i + 2];
-        x.w = half ? o[4 * (i ^ 1) + 3] : o[4 * i + 3];
-      }
-      *reinterpret_cast<uint4*>(row + ((c ^ (tok & 7)) << 4)) = x;
-    }
+    for (int i = 0; i < CH; ++i)
+      *reinterpret_cast<uint4*>(row + ((((c0 & 7) + i) ^ (tok & 7)) << 4)) =
+          make_uint4(scaled(o[4 * i], hi, lo), scaled(o[4 * i + 1], hi, lo), scaled(o[4 * i + 2], hi, lo), scaled(o[4 * i + 3], hi, lo));
   }
 };
 
+// One code for keys and values (`values`): the four roles' inner loops together have to stay in the instruction caches, and
+// are kept small for it.  Of every tile the warp takes the tokens 32 w .. 32 w + 31 (lane = token where scales are meant).
 template <int D, int FMT>
-__device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh, uint8_t* base, KvWalk<kKvTcRows> walk) {
+__device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh, uint8_t* base, KvWalk<kKvTcRows> walk, const bool values) {
   using C = Conv<D, FMT>;
-  const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - 8;        // this warp's tokens: 32 w .. 32 w + 31 of a tile
+  constexpr int G = C::N < 4 ? C::N : 4;                                  // pieces in registers; a tile is N / G groups of them
+  const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) & 3, c_tok = C::token(lane), c_piece = C::piece(lane);
   volatile int* abort = &sh.abort;
   const KvBatch& kb = p.kb;
+  const uint8_t* codes = (values ? p.v_codes : p.k_codes) + c_piece * 16;
+  const float* scales = values ? p.v_scales : p.k_scales;
+  const uint8_t* zeros = values ? p.v_zeros : p.k_zeros;
+  uint64_t* full_bar = values ? sh.v_full : sh.k_full;
+  uint64_t* empty_bar = values ? sh.v_empty : sh.k_empty;
+  uint8_t* tiles = base + (values ? Lay<D>::V : Lay<D>::K);
 
   KvPiece pc;
   bool have = walk.next(p, blockIdx.x, pc);
   int tile = have ? pc.t0 : 0;
-  auto settle = [&]() {                                                   // to the next tile that exists
+  // A tile two ahead: its page numbers are on their way while the codes of the one before are fetched.
+  struct Item { int page, place, head; uint32_t flags; };                 // flags: 1 tile exists, 2 token within the sequence, 4 new tokens
+  auto fetch = [&]() {
+    Item it{-1, 0, 0, 0u};
     while (have && tile >= pc.t1) {
       have = walk.next(p, blockIdx.x, pc);
       tile = have ? pc.t0 : 0;
     }
-  };
-  settle();
-
-  // One tile ahead: `slot` of the tile whose codes are loaded next (lane's token of each of its four 32-token parts).
-  int64_t slot[4];
-  bool draft_next = false;
-  auto locate = [&]() {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int pos = tile * kKvTile + i * 32 + lane;
-      slot[i] = -1;
+    if (have) {
+      const int pos = tile * kKvTile + w * 32 + lane;
+      it.head = pc.head;
+      it.flags = 1u | ((tile + 1) * kKvTile > pc.s.ctx ? 4u : 0u);
       if (pos < pc.s.len) {
         const int pi = p.page_shift >= 0 ? pos >> p.page_shift : pos / kb.page_size;
-        const int page = kb.page_table[(int64_t)walk.b * kb.pt_stride + pi];
-        if ((unsigned)page < (unsigned)kb.num_pages) slot[i] = ((int64_t)page * kb.hkv + pc.head) * kb.page_size + (pos - pi * kb.page_size);
+        it.place = pos - pi * kb.page_size;
+        it.page = __ldg(kb.page_table + (int64_t)walk.b * kb.pt_stride + pi);
+        it.flags |= 2u;
       }
-    }
-    draft_next = (tile + 1) * kKvTile > pc.s.ctx;
-  };
-  auto own = [&]() { return w == 0 ? slot[0] : w == 1 ? slot[1] : w == 2 ? slot[2] : slot[3]; };
-  auto load = [&](const uint8_t* codes, uint4 (&u)[C::N]) {
-    const int64_t mine = own();
-#pragma unroll
-    for (int i = 0; i < C::N; ++i) {
-      const int64_t s = __shfl_sync(0xffffffffu, mine, lane / C::CPT + i * C::TPI);
-      u[i] = make_uint4(0, 0, 0, 0);
-      if (s >= 0) u[i] = __ldg(reinterpret_cast<const uint4*>(codes + s * C::RB + (lane % C::CPT) * 16));
-    }
-  };
-  struct { float k[4], v[4]; uint32_t z, valid[4]; bool draft; } sc;
-  auto load_scales = [&]() {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sc.k[i] = slot[i] >= 0 ? __ldg(p.k_scales + slot[i]) : 0.f;
-      sc.v[i] = slot[i] >= 0 ? __ldg(p.v_scales + slot[i]) : 0.f;
-      sc.valid[i] = __ballot_sync(0xffffffffu, slot[i] >= 0);
-    }
-    sc.draft = draft_next;
-    sc.z = 0;
-    if (FMT == GL_KV_INT4) {
-      const int64_t s = own();
-      if (s >= 0) sc.z = (uint32_t)__ldg(p.k_zeros + s) | (uint32_t)__ldg(p.v_zeros + s) << 8;
-    }
-  };
-
-  uint4 ku[C::N], vu[C::N];
-  bool live = have;
-  if (live) {
-    locate();
-    load(p.k_codes, ku);
-    load(p.v_codes, vu);
-    load_scales();
-    ++tile;
-    settle();
-    if (have) locate();
-  }
-  for (int n = 0; live; ++n) {
-    const int st = n & 1;
-    const uint32_t parity = ((n >> 1) & 1) ^ 1;
-    // the tile's powers of two, by every warp alike
-    uint32_t kt = 0, vt = 0, kl = 0x7f7fffffu, vl = 0x7f7fffffu;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t kbits = __float_as_uint(sc.k[i]), vbits = __float_as_uint(sc.v[i]);
-      if (kbits - 1u < 0x7f7fffffu) { kt = max(kt, kbits); kl = min(kl, kbits); }       // positive and finite
-      if (vbits - 1u < 0x7f7fffffu) { vt = max(vt, vbits); vl = min(vl, vbits); }
-    }
-    kt = __reduce_max_sync(0xffffffffu, kt);
-    vt = __reduce_max_sync(0xffffffffu, vt);
-    kl = __reduce_min_sync(0xffffffffu, kl);
-    vl = __reduce_min_sync(0xffffffffu, vl);
-    const bool apart = (sc.draft && p.mask != nullptr) || (int)(kt >> 23) - (int)(kl >> 23) >= kSpread || (int)(vt >> 23) - (int)(vl >> 23) >= kSpread;
-    const int ke = apart ? 0 : pow2_above(kt) - kRoom<FMT>, ve = apart ? 0 : pow2_above(vt) - kRoom<FMT>;
-    const float k_own = w == 0 ? sc.k[0] : w == 1 ? sc.k[1] : w == 2 ? sc.k[2] : sc.k[3], v_own = w == 0 ? sc.v[0] : w == 1 ? sc.v[1] : w == 2 ? sc.v[2] : sc.v[3];
-    const bool v_bad = !(fabsf(v_own) < INFINITY), v_none = v_own < 1e-30f;
-    const uint32_t kr = !(fabsf(k_own) < INFINITY) ? 0x00007fffu : apart ? 0x00003c00u : split_half(k_own * pow2(-ke));
-    const uint32_t vr = v_bad || (apart && v_none) ? 0u : apart ? 0x00003c00u : split_half(v_own * pow2(-ve));
-    // Values that are not numbers: as P V' they would reach every row, so V' is 0 there and K' is NaN, which the rows that
-    // see the token keep.  (Codes that are e4m3's NaN only matter where some rows do not see the token.)
-    uint32_t bad = __ballot_sync(0xffffffffu, v_bad);
-    if (FMT == GL_KV_FP8 && sc.draft) {
-#pragma unroll
-      for (int i = 0; i < C::N; ++i) {
-        const uint32_t m = 0x7f7f7f7fu, one = 0x01010101u;
-        const bool nan = (((((vu[i].x & m) + one) | ((vu[i].y & m) + one) | ((vu[i].z & m) + one) | ((vu[i].w & m) + one)) & 0x80808080u) != 0);
-        const uint32_t who = __ballot_sync(0xffffffffu, nan);
-#pragma unroll
-        for (int t = 0; t < C::TPI; ++t)
-          if ((who >> (t * C::CPT)) & ((1u << C::CPT) - 1u)) bad |= 1u << (t + i * C::TPI);
-      }
-    }
-    const uint32_t zk = 0x6400u + (sc.z & 255u), zv = 0x6400u + (sc.z >> 8);
-
-    if (n >= 2 && !warp_wait(&sh.k_empty[st], parity, abort)) return;
-    if (lane == 0 && w == 0) {
-      Meta& m = sh.meta[n % kMeta];
-      m.apart = apart;
-      m.ks = pow2(ke);
-      m.vs_log2 = (float)ve;
-      m.vs_inv = pow2(-ve);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) m.valid[i] = sc.valid[i];
-    }
-    if (apart) {
-      Meta& m = sh.meta[n % kMeta];
-      const float v = v_none ? 1e-30f : v_own;
-      m.col_ks[w * 32 + lane] = k_own;
-      m.col_lv[w * 32 + lane] = __log2f(v);
-      m.col_rv[w * 32 + lane] = __frcp_rn(v);
-    }
-    uint8_t* kt_s = base + Lay<D>::K + st * Lay<D>::TILE;
-    uint8_t* vt_s = base + Lay<D>::V + st * Lay<D>::TILE;
-#pragma unroll
-    for (int i = 0; i < C::N; ++i) {
-      const int t = lane / C::CPT + i * C::TPI;
-      const uint32_t r = __shfl_sync(0xffffffffu, kr, t);
-      uint32_t z = 0;
-      if (FMT == GL_KV_INT4) { z = __shfl_sync(0xffffffffu, zk, t); z |= z << 16; }
-      C::put(kt_s, w * 32 + t, lane % C::CPT, ku[i], r, z, false, (bad >> t) & 1u);
-    }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&sh.k_full[st]);
-    const bool more = have;
-    if (more) {
-      load(p.k_codes, ku);
-      load_scales();
-    }
-    if (n >= 2 && !warp_wait(&sh.v_empty[st], parity, abort)) return;
-#pragma unroll
-    for (int i = 0; i < C::N; ++i) {
-      const int t = lane / C::CPT + i * C::TPI;
-      const uint32_t r = __shfl_sync(0xffffffffu, vr, t);
-      uint32_t z = 0;
-      if (FMT == GL_KV_INT4) { z = __shfl_sync(0xffffffffu, zv, t); z |= z << 16; }
-      C::put(vt_s, w * 32 + t, lane % C::CPT, vu[i], r, z, (bad >> t) & 1u, false);
-    }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&sh.v_full[st]);
-    if (more) {
-      load(p.v_codes, vu);
       ++tile;
-      settle();
-      if (have) locate();
     }
-    live = more;
+    return it;
+  };
+  auto slot_of = [&](const Item& it) -> int64_t {
+    return (it.flags & 2u) && (unsigned)it.page < (unsigned)kb.num_pages ? ((int64_t)it.page * kb.hkv + it.head) * kb.page_size + it.place : -1;
+  };
+  auto take = [&](int64_t slot, int piece) {
+    const int64_t s = __shfl_sync(0xffffffffu, slot, c_tok + piece * C::TPI);
+    return s >= 0 ? __ldg(reinterpret_cast<const uint4*>(codes + s * C::RB)) : make_uint4(0, 0, 0, 0);
+  };
+
+  Item nxt = fetch();
+  if (!(nxt.flags & 1u)) return;
+  int64_t slot = slot_of(nxt);
+  uint32_t flags = nxt.flags;
+  nxt = fetch();
+  uint4 u[G];
+#pragma unroll
+  for (int i = 0; i < G; ++i) u[i] = take(slot, i);
+  float scale = slot >= 0 ? __ldg(scales + slot) : 0.f;
+  uint32_t zero = FMT == GL_KV_INT4 && slot >= 0 ? __ldg(zeros + slot) : 0u;
+
+#pragma unroll 1
+  for (int n = 0; flags & 1u; ++n) {
+    const int st = n & 1;
+    const bool draft = flags & 4u;
+    // the power of two, and whether the scales are near enough to each other
+    const uint32_t bits = __float_as_uint(scale);
+    const bool plain = bits - 1u < 0x7f7fffffu;                          // positive and finite
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, plain ? bits : 0u), lo = __reduce_min_sync(0xffffffffu, plain ? bits : 0x7f7fffffu);
+    const bool apart = (draft && p.mask != nullptr) || (int)(hi >> 23) - (int)(lo >> 23) >= kSpread;
+    const int e = apart ? 0 : pow2_above(hi) - kRoom<FMT>;
+    const bool number = fabsf(scale) < INFINITY, none = apart && scale < 1e-30f;
+    const uint32_t valid = __ballot_sync(0xffffffffu, slot >= 0);
+    // Values that are not numbers would reach every row through P V', so V' is 0 there, and the exponent is NaN, which only the
+    // rows that see the token meet.  (e4m3's NaN codes matter where some rows do not see the token.)
+    uint32_t bad = values ? __ballot_sync(0xffffffffu, !number) : 0u;
+    const uint32_t ratio = !number ? (values ? 0u : 0x00007fffu) : values && none ? 0u : apart ? 0x00003c00u : split_half(scale * pow2(-e));
+    const uint32_t zz = (0x6400u + zero) * 0x10001u;
+    const int64_t slot_next = slot_of(nxt);
+
+    if (n >= 2 && !warp_wait(&empty_bar[st], ((n >> 1) & 1) ^ 1, abort)) return;
+    uint8_t* dst = tiles + st * Lay<D>::TILE;
+#pragma unroll 1
+    for (int g = 0; g < C::N; g += G) {
+      const bool last = g + G >= C::N;                                    // then the pieces of the next tile follow
+      const int64_t from = last ? slot_next : slot;
+      const int base_piece = last ? 0 : g + G;
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const int t = c_tok + (g + i) * C::TPI;
+        if (FMT == GL_KV_FP8 && values && draft) {
+          const uint32_t m = 0x7f7f7f7fu, one = 0x01010101u;
+          const bool nan = (((((u[i].x & m) + one) | ((u[i].y & m) + one) | ((u[i].z & m) + one) | ((u[i].w & m) + one)) & 0x80808080u) != 0);
+          const uint32_t who = __reduce_or_sync(0xffffffffu, nan ? 1u << t : 0u);
+          if ((who >> t) & 1u) u[i] = make_uint4(0, 0, 0, 0);
+          bad |= who;
+        }
+        const uint32_t r = __shfl_sync(0xffffffffu, ratio, t), z = FMT == GL_KV_INT4 ? __shfl_sync(0xffffffffu, zz, t) : 0u;
+        C::put(dst, w * 32 + t, c_piece, u[i], r, z);
+        u[i] = take(from, base_piece + i);
+      }
+    }
+    Meta& m = sh.meta[n % kMeta];
+    if (lane == 0) {
+      if (values) {
+        m.vs_log2[w] = (float)e;
+        m.vs_inv[w] = pow2(-e);
+        m.v_apart[w] = apart || bad;
+      } else {
+        m.ks[w] = pow2(e);
+        m.k_apart[w] = apart;
+        m.valid[w] = valid;
+      }
+    }
+    if (apart || bad) {
+      const float v = apart ? (none ? 1e-30f : scale) : pow2(e);         // (folded already: the power of two is left)
+      const bool is_bad = (bad >> lane) & 1u;
+      if (values) {
+        m.col_lv[w * 32 + lane] = is_bad ? __int_as_float(0x7fc00000) : __log2f(v);
+        m.col_rv[w * 32 + lane] = __frcp_rn(v);
+      } else {
+        m.col_ks[w * 32 + lane] = scale;
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&full_bar[st]);
+    flags = nxt.flags;
+    slot = slot_next;
+    if (flags & 1u) {
+      scale = slot >= 0 ? __ldg(scales + slot) : 0.f;
+      if (FMT == GL_KV_INT4) zero = slot >= 0 ? __ldg(zeros + slot) : 0u;
+      nxt = fetch();
+    }
   }
 }
 
@@ -317,6 +283,9 @@ template <int D>
 __device__ __forceinline__ void mma_role(const KvAttendParams& p, Shared& sh, uint32_t base, KvWalk<kKvTcRows> walk, uint32_t idesc_s, uint32_t idesc_o) {
   volatile int* abort = &sh.abort;
   const uint32_t tm = sh.tmem;
+  // descriptors as halves: the high words are constant, the low words step with the address
+  const uint64_t qd = smem_desc_sw128(base + Lay<D>::Q), kd = smem_desc_sw128(base + Lay<D>::K), vd = desc_mn(base + Lay<D>::V);
+  const uint32_t q_lo = (uint32_t)qd, k_lo = (uint32_t)kd, k_hi = (uint32_t)(kd >> 32), v_lo = (uint32_t)vd, v_hi = (uint32_t)(vd >> 32);
   KvPiece pc;
   int n0 = 0;                                  // tiles of earlier pieces
   uint32_t q_phase = 0, p_phase[2] = {0, 0};
@@ -329,12 +298,12 @@ __device__ __forceinline__ void mma_role(const KvAttendParams& p, Shared& sh, ui
       const int s = e & 1, j = n0 + (both ? e >> 1 : e), st = j & 1;
       if ((!both || s == 0) && !mbar_wait_spin(&sh.k_full[st], (j >> 1) & 1, abort, nullptr, 0)) return false;
       tc_fence_after();
-      const uint32_t q = base + Lay<D>::Q + s * Lay<D>::TILE, k = base + Lay<D>::K + st * Lay<D>::TILE;
+      const uint32_t q = q_lo + s * (Lay<D>::TILE >> 4), k = k_lo + st * (Lay<D>::TILE >> 4);
+#pragma unroll 1
+      for (int half = 0; half < D / 64; ++half)
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        const uint32_t off = (kk >> 2) * Lay<D>::HALF + (kk & 3) * 32;
-        mma_ss<KIND_F16>(tm + s * 128, smem_desc_sw128(q + off), smem_desc_sw128(k + off), idesc_s, kk > 0);
-      }
+        for (int kk = 0; kk < 4; ++kk)
+          mma_ss_f16_lohi(tm + s * 128, q + half * (Lay<D>::HALF >> 4) + kk * 2, k + half * (Lay<D>::HALF >> 4) + kk * 2, k_hi, idesc_s, half + kk > 0);
       tc_commit(&sh.s_full[s]);
       if (!both || s == 1) tc_commit(&sh.k_empty[st]);
       return true;
@@ -351,10 +320,12 @@ __device__ __forceinline__ void mma_role(const KvAttendParams& p, Shared& sh, ui
       if (!mbar_wait_spin(&sh.p_full[s], p_phase[s], abort, nullptr, 0)) return;
       p_phase[s] ^= 1;
       tc_fence_after();
-      const uint32_t v = base + Lay<D>::V + st * Lay<D>::TILE;
+      const uint32_t v = v_lo + st * (Lay<D>::TILE >> 4);
+#pragma unroll 1
+      for (int k2 = 0; k2 < 8; k2 += 4)
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk)
-        mma_ts_f16(tm + 256 + s * D, tm + s * 128 + kk * 8, desc_mn(v + kk * 2048), idesc_o, e >= 2 || kk > 0);
+        for (int kk = k2; kk < k2 + 4; ++kk)
+          mma_ts_f16_lohi(tm + 256 + s * D, tm + s * 128 + kk * 8, v + kk * 128, v_hi, idesc_o, e >= 2 || kk > 0);
       if (!both || s == 1) tc_commit(&sh.v_empty[st]);
       if (e + 2 >= events) tc_commit(&sh.o_full[s]);
       else if (!scores(e + 2)) return;
@@ -426,14 +397,14 @@ __device__ __forceinline__ void stream_role(const KvAttendParams& p, Shared& sh,
       for (int i = 0; i < mine && ok; ++i) {
         const int j = both ? i : 2 * i + s;
         const Meta& meta = sh.meta[(n0 + j) % kMeta];
-        ok = warp_wait(&sh.s_full[s], s_phase, abort);
+        ok = warp_wait(&sh.s_full[s], s_phase, abort) && warp_wait(&sh.v_full[(n0 + j) & 1], ((n0 + j) >> 1) & 1, abort);     // (the values' scales)
         if (!ok) break;
         s_phase ^= 1;
         tc_fence_after();
         const int tile0 = (pc.t0 + j) * kKvTile;
-        const uint4 vld = make_uint4(meta.valid[0], meta.valid[1], meta.valid[2], meta.valid[3]);
-        const bool full = meta.apart == 0 && (vld.x & vld.y & vld.z & vld.w) == 0xffffffffu && tile0 + kKvTile <= pc.s.ctx + (p.mask == nullptr ? t_lo + 1 : 0);
-        const float a = qs * meta.ks, lv = meta.vs_log2;
+        const uint4 vld = *reinterpret_cast<const uint4*>(meta.valid), ka = *reinterpret_cast<const uint4*>(meta.k_apart), va = *reinterpret_cast<const uint4*>(meta.v_apart);
+        const bool full = (ka.x | ka.y | ka.z | ka.w | va.x | va.y | va.z | va.w) == 0 && (vld.x & vld.y & vld.z & vld.w) == 0xffffffffu &&
+                          tile0 + kKvTile <= pc.s.ctx + (p.mask == nullptr ? t_lo + 1 : 0);
         uint32_t seen[4] = {vld.x, vld.y, vld.z, vld.w};
         if (!full) {
 #pragma unroll
@@ -451,22 +422,23 @@ __device__ __forceinline__ void stream_role(const KvAttendParams& p, Shared& sh,
             }
           }
         }
-        const bool apart = meta.apart != 0;
-        auto exponent = [&](float sc, int col) { return apart ? fmaf(sc * meta.col_ks[col], qs, meta.col_lv[col]) : fmaf(sc, a, lv); };
         // ---- the tile's maximum.  (The paths for tiles that are not full are rolled up: unrolled, the kernel outgrew the
-        // instruction cache and ran at a fifth of its speed.)
-        float top = -INFINITY;
-        uint32_t x[2][32];
+        // instruction cache and ran at less than half its speed.)
+        auto exponent = [&](float sc, int col) {
+          const int w = col >> 5;
+          return (meta.k_apart[w] ? sc * meta.col_ks[col] * qs : sc * (qs * meta.ks[w])) + (meta.v_apart[w] ? meta.col_lv[col] : meta.vs_log2[w]);
+        };
+        float t_top = -INFINITY;
         if (full) {
+          uint32_t x[32];
 #pragma unroll 1
-          for (int h = 0; h < 128; h += 64) {
-            tmem_ld_32x32_issue(ts + h, x[0]);
-            tmem_ld_32x32_issue(ts + h + 32, x[1]);
-            tmem_ld_wait();
-            tmem_ld_fence(x[0]);
-            tmem_ld_fence(x[1]);
+          for (int h = 0; h < 4; ++h) {
+            tmem_ld_32x32(ts + 32 * h, x);
+            tmem_ld_fence(x);
+            float top = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < 32; ++k) top = fmaxf(top, fmaxf(__uint_as_float(x[0][k]), __uint_as_float(x[1][k])));
+            for (int k = 0; k < 32; k += 2) top = fmaxf(top, fmaxf(__uint_as_float(x[k]), __uint_as_float(x[k + 1])));
+            t_top = fmaxf(t_top, fmaf(top, qs * meta.ks[h], meta.vs_log2[h]));
           }
         } else {
 #pragma unroll 1
@@ -475,16 +447,16 @@ __device__ __forceinline__ void stream_role(const KvAttendParams& p, Shared& sh,
             tmem_ld_8(ts + c, y);
             const uint32_t sw = (c < 64 ? (c < 32 ? seen[0] : seen[1]) : (c < 96 ? seen[2] : seen[3])) >> (c & 31);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) top = (sw >> k) & 1u ? fmaxf(top, exponent(__uint_as_float(y[k]), c + k)) : top;
+            for (int k = 0; k < 8; ++k) t_top = (sw >> k) & 1u ? fmaxf(t_top, exponent(__uint_as_float(y[k]), c + k)) : t_top;
           }
         }
-        const float t_top = full ? fmaf(top, a, lv) : top;
         const bool raise = t_top > m_used + kRaise || (m_used == -INFINITY && t_top != -INFINITY);
         if (__any_sync(0xffffffffu, raise)) {
           const float m_new = fmaxf(m_used, t_top), f = m_used == m_new ? 1.f : kv_exp2(m_used - m_new);
           l *= f;
           m_used = m_new;
           if (i > 0) {                                                // (s_full: the products before this tile's scores are done)
+            uint32_t x[1][32];
 #pragma unroll 1
             for (int d = 0; d < D; d += 32) {
               tmem_ld_32x32(to + d, x[0]);
@@ -496,43 +468,41 @@ __device__ __forceinline__ void stream_role(const KvAttendParams& p, Shared& sh,
           }
         }
         // ---- weights, over the scores
-        const float to_p = m_used == -INFINITY ? 0.f : kOff - m_used, sub = lv + to_p, inv_vs = meta.vs_inv;
-        float sum = 0.f;
+        const float to_p = m_used == -INFINITY ? 0.f : kOff - m_used;
         if (full) {
+          uint32_t x[32];
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            tmem_ld_32x32_issue(ts + h * 64, x[0]);
-            tmem_ld_32x32_issue(ts + h * 64 + 32, x[1]);
-            tmem_ld_wait();
-            tmem_ld_fence(x[0]);
-            tmem_ld_fence(x[1]);
-            uint32_t pk[32];
-            float s1 = 0.f;
+          for (int h = 0; h < 4; ++h) {
+            tmem_ld_32x32(ts + 32 * h, x);
+            tmem_ld_fence(x);
+            const float a = qs * meta.ks[h], sub = meta.vs_log2[h] + to_p;
+            float s0 = 0.f, s1 = 0.f;
+            uint32_t pk[16];
 #pragma unroll
-            for (int q = 0; q < 2; ++q)
-#pragma unroll
-              for (int k = 0; k < 32; k += 2) {
-                const float e0 = kv_exp2(fmaf(__uint_as_float(x[q][k]), a, sub)), e1 = kv_exp2(fmaf(__uint_as_float(x[q][k + 1]), a, sub));
-                sum += e0;
-                s1 += e1;
-                const __half2 hh = __floats2half2_rn(e0, e1);
-                pk[q * 16 + (k >> 1)] = *reinterpret_cast<const uint32_t*>(&hh);
-              }
-            sum += s1;
-            tmem_st_32x32(ts + h * 32, pk);
+            for (int k = 0; k < 32; k += 2) {
+              const float e0 = kv_exp2(fmaf(__uint_as_float(x[k]), a, sub)), e1 = kv_exp2(fmaf(__uint_as_float(x[k + 1]), a, sub));
+              s0 += e0;
+              s1 += e1;
+              const __half2 hh = __floats2half2_rn(e0, e1);
+              pk[k >> 1] = *reinterpret_cast<const uint32_t*>(&hh);
+            }
+            l = fmaf(s0 + s1, meta.vs_inv[h], l);
+            tmem_st_16(ts + h * 16, pk);                              // (columns whose scores have been read)
           }
-          sum *= inv_vs;
+          tmem_st_wait();
         } else {
 #pragma unroll 1
           for (int c = 0; c < 128; c += 8) {
             uint32_t y[8], pk[4];
             tmem_ld_8(ts + c, y);
             const uint32_t sw = (c < 64 ? (c < 32 ? seen[0] : seen[1]) : (c < 96 ? seen[2] : seen[3])) >> (c & 31);
+            const bool apart = meta.v_apart[c >> 5] != 0;
+            const float inv_vs = meta.vs_inv[c >> 5];
             float e[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               e[k] = (sw >> k) & 1u ? kv_exp2(exponent(__uint_as_float(y[k]), c + k) + to_p) : 0.f;
-              sum += (sw >> k) & 1u ? e[k] * (apart ? meta.col_rv[c + k] : inv_vs) : 0.f;
+              l += (sw >> k) & 1u ? e[k] * (apart ? meta.col_rv[c + k] : inv_vs) : 0.f;
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -542,7 +512,6 @@ __device__ __forceinline__ void stream_role(const KvAttendParams& p, Shared& sh,
             tmem_st_4(ts + c / 2, pk);
           }
         }
-        l += sum;
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.p_full[s]);
@@ -667,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tc_kernel(const KvAtten
     sh.abort = sh.never = 0;
     fence_barrier_init();
   }
-  if (warp == 12) tmem_alloc(&sh.tmem, 512);
+  if (warp == 16) tmem_alloc(&sh.tmem, 512);
   gl_launch_dependents();
   gl_grid_dependency_wait();
   KvWalk<kKvTcRows> walk;
@@ -677,16 +646,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tc_kernel(const KvAtten
   tc_fence_after();
 
   // Every wait is bounded; one that gives up ends all roles, and the rows that it leaves unfinished become NaN.
-  // Registers: 512 threads are launched with 128 each; 3 x 152 + 56 = 512 are what they are given again.
+  // Registers: 640 threads are launched with 96 each; 2 x 128 + 2 x 88 + 48 = 480 = 5 x 96 are shared out again.
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
     stream_role<D, T>(p, sh, base, walk);
-  } else if (warp < 12) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
-    convert_role<D, FMT>(p, sh, base, walk);
+  } else if (warp < 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    convert_role<D, FMT>(p, sh, base, walk, warp >= 12);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (threadIdx.x == 12 * 32) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    if (threadIdx.x == 16 * 32) {
       mma_role<D>(p, sh, smem_u32(base), walk, idesc_s, idesc_o);
       // nothing of this block's is in flight when the TMEM goes back
       tc_commit(&sh.drain);
@@ -697,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tc_kernel(const KvAtten
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(sh.tmem, 512);
+  if (warp == 16) tmem_dealloc(sh.tmem, 512);
 }
 
 template <int D, int FMT, typename T>
