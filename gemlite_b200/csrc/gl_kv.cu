@@ -12,6 +12,9 @@ int gl_kv_check(const char* fn, const gl_kv_args* a) {
   if (a->num_pages <= 0 || a->page_size <= 0 || a->n_kv_heads <= 0 || a->batch < 0 || a->max_pages < 0 || a->n_tokens < 0 || a->max_len < 0 || a->max_new < 0)
     GL_FAIL(GL_E_INVALID, "%s: bad size (pages %d x %d, kv heads %d, batch %d, table columns %d, tokens %d)", fn, a->num_pages, a->page_size,
             a->n_kv_heads, a->batch, a->max_pages, a->n_tokens);
+  // slots are 32-bit numbers: 2^32 rows of keys and values, 74 bytes at least, are more than the GPU's memory
+  if ((uint64_t)a->num_pages * (uint64_t)a->n_kv_heads > 0xfffffffeull / (uint64_t)a->page_size)
+    GL_FAIL(GL_E_UNSUPPORTED, "%s: %d pages of %d heads x %d tokens (at most 2^32 - 2 rows)", fn, a->num_pages, a->n_kv_heads, a->page_size);
   if (!a->k_codes || !a->v_codes || !a->k_scales || !a->v_scales) GL_FAIL(GL_E_INVALID, "%s: null cache pointer", fn);
   if (((uintptr_t)a->k_codes | (uintptr_t)a->v_codes) & 15) GL_FAIL(GL_E_INVALID, "%s: codes must be 16-byte aligned", fn);
   if (a->format == GL_KV_INT4 && (!a->k_zeros || !a->v_zeros)) GL_FAIL(GL_E_INVALID, "%s: the 4-bit cache needs zeros", fn);

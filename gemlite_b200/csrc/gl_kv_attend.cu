@@ -145,15 +145,13 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 3 : 2) kv_attend_mma_ke
     const int tiles = c1 > c0 ? (c1 - c0 + kTile - 1) / kTile : 0;
     const int mine = (tiles - warp + kWarps - 1) / kWarps;              // tiles warp, warp + 4, ..
 
-    auto slot_of = [&](int i) -> int64_t {                              // lane's token of the warp's i-th tile
+    auto slot_of = [&](int i) -> uint32_t {                             // lane's token of the warp's i-th tile
       const int pos = c0 + (warp + i * kWarps) * kTile + lane;
-      if (i >= mine || pos >= c1) return -1;
+      if (i >= mine || pos >= c1) return kNoSlot;
       const int pi = p.page_shift >= 0 ? pos >> p.page_shift : pos / kb.page_size;
-      const int page = kb.page_table[pt_row + pi];
-      if ((unsigned)page >= (unsigned)kb.num_pages) return -1;
-      return ((int64_t)page * kb.hkv + kvh) * kb.page_size + (pos - pi * kb.page_size);
+      return kv_slot32(kb, kb.page_table[pt_row + pi], kvh, pos - pi * kb.page_size);
     };
-    int64_t slot_next = slot_of(0);
+    uint32_t slot_next = slot_of(0);
     uint32_t z_pend = 0;
     int z_stage = -1;
     auto put_zeros = [&]() {
@@ -168,34 +166,35 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 3 : 2) kv_attend_mma_ke
       if (i < mine) {
         const int st = i % kStages;
         const uint32_t at = ring_u + st * S::STAGE;
-        const int64_t slot = slot_next;
+        const uint32_t slot = slot_next, slot0 = __shfl_sync(0xffffffffu, slot, 0);
+        const bool live = slot != kNoSlot;
         slot_next = slot_of(i + 1);
-        const int64_t slot0 = __shfl_sync(0xffffffffu, slot, 0);
-        if (__all_sync(0xffffffffu, slot == slot0 + lane && slot0 >= 0)) {         // 32 rows in a row: a tile inside one page
-          const uint8_t *ks = p.k_codes + slot0 * RB + lane * 16, *vs = p.v_codes + slot0 * RB + lane * 16;
+        if (__all_sync(0xffffffffu, slot == slot0 + lane && live)) {              // 32 rows in a row: a tile inside one page
+          const uint8_t *ks = p.k_codes + (int64_t)slot0 * RB + lane * 16, *vs = p.v_codes + (int64_t)slot0 * RB + lane * 16;
 #pragma unroll
           for (int k = 0; k < CPT; ++k) {
             const int t = lane / CPT + k * (32 / CPT), ch = lane % CPT;
             cp_async16(at + S::K_AT + k_place<RB>(t, ch), ks + k * 512, true);
             cp_async16(at + S::V_AT + v_place<RB>(t, ch), vs + k * 512, true);
           }
-        } else
+        } else {
 #pragma unroll
-        for (int k = 0; k < CPT; ++k) {
-          const int t = lane / CPT + k * (32 / CPT), ch = lane % CPT;
-          const int64_t s = __shfl_sync(0xffffffffu, slot, t);
-          const int64_t off = s < 0 ? 0 : s * RB + ch * 16;
-          cp_async16(at + S::K_AT + k_place<RB>(t, ch), p.k_codes + off, s >= 0);
-          cp_async16(at + S::V_AT + v_place<RB>(t, ch), p.v_codes + off, s >= 0);
+          for (int k = 0; k < CPT; ++k) {
+            const int t = lane / CPT + k * (32 / CPT), ch = lane % CPT;
+            const uint32_t s = __shfl_sync(0xffffffffu, slot, t);
+            const int64_t off = s == kNoSlot ? 0 : (int64_t)s * RB + ch * 16;
+            cp_async16(at + S::K_AT + k_place<RB>(t, ch), p.k_codes + off, s != kNoSlot);
+            cp_async16(at + S::V_AT + v_place<RB>(t, ch), p.v_codes + off, s != kNoSlot);
+          }
         }
-        const int64_t so = slot < 0 ? 0 : slot;
-        cp_async4(at + S::KS_AT + lane * 4, p.k_scales + so, slot >= 0);
-        cp_async4(at + S::VS_AT + lane * 4, p.v_scales + so, slot >= 0);
+        const uint32_t so = live ? slot : 0u;
+        cp_async4(at + S::KS_AT + lane * 4, p.k_scales + so, live);
+        cp_async4(at + S::VS_AT + lane * 4, p.v_scales + so, live);
         if (FMT == GL_KV_INT4) {
-          z_pend = slot >= 0 ? (uint32_t)p.k_zeros[so] | (uint32_t)p.v_zeros[so] << 8 : 0u;
+          z_pend = live ? (uint32_t)p.k_zeros[so] | (uint32_t)p.v_zeros[so] << 8 : 0u;
           z_stage = st;
         }
-        const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);
+        const uint32_t there = __ballot_sync(0xffffffffu, live);
         if (lane == 0) *reinterpret_cast<uint32_t*>(ring + st * S::STAGE + S::VALID_AT) = there;
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -452,13 +451,15 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 3 : 2) kv_attend_mma_ke
   }
 }
 
-// Joins the parts of the units that block borders cut.  Block (i, y) looks after border i + 1 if it is the first one in its
-// unit: rows y, y + gridDim.y, .., warp w takes parts w, w + 8, ..
+// Joins the parts of the units that block borders cut.  Blocks (i, *) look after border i + 1 if it is the first one in its
+// unit.  Few parts (a border or two in a unit): a warp per row; many (one long sequence): a block per row, warp w takes parts
+// w, w + 8, ..
 template <int ROWS, int D, typename T>
 __global__ void __launch_bounds__(256) kv_attend_join_kernel(const KvAttendParams p) {
   __shared__ KvPlaceScratch place_scratch;
   __shared__ float4 acc_s[8][D / 4];
-  __shared__ float red[8];
+  __shared__ float2 red[8];
+  constexpr int V = D / 32;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, border = blockIdx.x + 1;
   gl_launch_dependents();
   gl_grid_dependency_wait();
@@ -473,50 +474,63 @@ __global__ void __launch_bounds__(256) kv_attend_join_kernel(const KvAttendParam
   if (i0 != border - 1) return;                                  // an earlier border of the unit does the work
   const int head = u / s.blocks, row0 = kv_row_block(u - head * s.blocks, s.blocks) * ROWS, rows = min(ROWS, s.new_b * p.group - row0);
   auto part = [&](int i) { return (int64_t)(2 * i + (i == i0 ? 1 : 0)) * ROWS; };
+  const bool few = i1 - i0 < 16;
+  const int first = few ? i0 : i0 + warp, step = few ? 1 : 8;
 
-  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+  for (int r = few ? blockIdx.y * 8 + warp : blockIdx.y; r < rows; r += gridDim.y * (few ? 8 : 1)) {
+    // maximum of the parts that saw anything (a sum of NaN counts)
     float top = -INFINITY;
-    for (int i = i0 + tid; i <= i1; i += 256) {
+    for (int i = few ? i0 + lane : i0 + tid; i <= i1; i += few ? 32 : 256) {
       const float2 ml = p.part_ml[part(i) + r];
       if (ml.y != 0.f) top = fmaxf(top, ml.x);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) red[warp] = top;
-    __syncthreads();
+    if (!few) {
+      if (lane == 0) red[warp].x = top;
+      __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; ++w) top = fmaxf(top, red[w]);
-    __syncthreads();
-    constexpr int V = D / 32;
+      for (int w = 0; w < 8; ++w) top = fmaxf(top, red[w].x);
+    }
     float acc[V] = {};
     float l = 0.f;
 #pragma unroll 4
-    for (int i = i0 + warp; i <= i1; i += 8) {
+    for (int i = first; i <= i1; i += step) {
       const float2 ml = p.part_ml[part(i) + r];
-      if (ml.y == 0.f) continue;
-      const float f = ml.x == -INFINITY ? ml.y : kv_exp2(ml.x - top);    // -inf with a sum: the sum is NaN
+      const float f = ml.y == 0.f ? 0.f : ml.x == -INFINITY ? ml.y : kv_exp2(ml.x - top);    // -inf with a sum: the sum is NaN
+      float x[V];
+      if constexpr (V == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p.part_o + (part(i) + r) * D + lane * V);
+      else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(p.part_o + (part(i) + r) * D + lane * V);
       l += ml.y * f;
-      const float* src = p.part_o + (part(i) + r) * D + lane * V;
 #pragma unroll
-      for (int j = 0; j < V; ++j) acc[j] += src[j] * f;
+      for (int j = 0; j < V; ++j) acc[j] += ml.y == 0.f ? 0.f : x[j] * f;
     }
+    const int rr = row0 + r, t = rr / p.group;
+    T* dst = reinterpret_cast<T*>(p.out) + ((int64_t)(s.first + t) * p.hq + head * p.group + (rr - t * p.group)) * D;
+    if (!few) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) reinterpret_cast<float*>(acc_s[warp])[lane * V + j] = acc[j];
-    if (lane == 0) red[warp] = l;
-    __syncthreads();
-    if (tid < D / 4) {
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-      l = 0.f;
+      for (int j = 0; j < V; ++j) reinterpret_cast<float*>(acc_s[warp])[lane * V + j] = acc[j];
+      __syncthreads();                                           // (everybody has read the maxima)
+      if (lane == 0) red[warp].y = l;
+      __syncthreads();
+      if (tid < D / 4) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        l = 0.f;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        const float4 x = acc_s[w][tid];
-        a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
-        l += red[w];
+        for (int w = 0; w < 8; ++w) {
+          const float4 x = acc_s[w][tid];
+          a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+          l += red[w].y;
+        }
+        kv_store4<T>(dst + tid * 4, a, l);
       }
-      const int rr = row0 + r, t = rr / p.group;
-      kv_store4<T>(reinterpret_cast<T*>(p.out) + ((int64_t)(s.first + t) * p.hq + head * p.group + (rr - t * p.group)) * D + tid * 4, a, l);
+      __syncthreads();
+    } else {
+      const float q = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] = l == 0.f ? 0.f : acc[j] * q;
+      kv_store_n<T, V>(dst + lane * V, acc);
     }
-    __syncthreads();
   }
 }
 
@@ -541,7 +555,7 @@ int launch_fmt(const KvAttendParams& p, int fmt, int mt, cudaStream_t st) {
 }
 template <int ROWS, int D, typename T>
 int launch_join(const KvAttendParams& p, int live_rows, cudaStream_t st) {
-  const int y = live_rows < 64 ? live_rows : 64;
+  const int y = live_rows < 16 ? live_rows : 16;
   GL_CUDA_CHECK(gl_launch_pdl(kv_attend_join_kernel<ROWS, D, T>, dim3((unsigned)(p.blocks - 1), (unsigned)y), dim3(256), 0, st, p));
   return GL_OK;
 }

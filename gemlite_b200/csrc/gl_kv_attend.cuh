@@ -26,6 +26,12 @@ template <typename T> struct IsHalf { static constexpr bool value = false; };
 template <> struct IsHalf<__half> { static constexpr bool value = true; };
 
 #ifdef __CUDACC__
+// row of a token's (page, head, place) in the cache as a 32-bit number (gl_kv_check: there are fewer than 2^32 - 1)
+constexpr uint32_t kNoSlot = 0xffffffffu;
+__device__ __forceinline__ uint32_t kv_slot32(const KvBatch& kb, int page, int head, int place) {
+  return (unsigned)page < (unsigned)kb.num_pages ? ((uint32_t)page * (uint32_t)kb.hkv + (uint32_t)head) * (uint32_t)kb.page_size + (uint32_t)place : kNoSlot;
+}
+
 // ---- how the work is dealt out
 // A unit is ROWS query rows (token, head of the group) of one kv head of one sequence; it is worked through in tiles of kKvTile cached
 // tokens.  All units' tiles stand in one line (sequence, kv head, row block, tile), and block i of n takes the i-th of n
@@ -200,19 +206,24 @@ __device__ __forceinline__ uint32_t kv_nibbles(uint32_t w, uint32_t zero) {
   const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&u), *reinterpret_cast<__half2*>(&zero));
   return *reinterpret_cast<const uint32_t*>(&x);
 }
+// two fp32 -> a pair of T
+template <typename T> __device__ __forceinline__ uint32_t kv_pair(float a, float b) {
+  if constexpr (IsHalf<T>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <typename T, int N> __device__ __forceinline__ void kv_store_n(T* dst, const float (&v)[N]) {
+  if constexpr (N == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(kv_pair<T>(v[0], v[1]), kv_pair<T>(v[2], v[3]));
+  else *reinterpret_cast<uint32_t*>(dst) = kv_pair<T>(v[0], v[1]);
+}
 // a / l, rounded once to 16 bits; a row that saw nothing (l = 0) gives zeros
 template <typename T> __device__ __forceinline__ void kv_store4(T* dst, float4 a, float l) {
   const float r = l == 0.f ? 0.f : 1.f / l;
-  uint32_t lo, hi;
-  if constexpr (IsHalf<T>::value) {
-    const __half2 x = __floats2half2_rn(a.x * r, a.y * r), y = __floats2half2_rn(a.z * r, a.w * r);
-    lo = *reinterpret_cast<const uint32_t*>(&x);
-    hi = *reinterpret_cast<const uint32_t*>(&y);
-  } else {
-    const __nv_bfloat162 x = __floats2bfloat162_rn(a.x * r, a.y * r), y = __floats2bfloat162_rn(a.z * r, a.w * r);
-    lo = *reinterpret_cast<const uint32_t*>(&x);
-    hi = *reinterpret_cast<const uint32_t*>(&y);
-  }
-  *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+  const float v[4] = {l == 0.f ? 0.f : a.x * r, l == 0.f ? 0.f : a.y * r, l == 0.f ? 0.f : a.z * r, l == 0.f ? 0.f : a.w * r};
+  kv_store_n<T, 4>(dst, v);
 }
 #endif

@@ -99,6 +99,28 @@ __device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&r)[1
                  "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// two fp32 operations per instruction
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // a bounded wait of a whole warp: its lanes go on together, or give up together
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, nullptr, 0));
@@ -183,24 +205,33 @@ __device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh
     }
     return it;
   };
-  auto slot_of = [&](const Item& it) -> int64_t {
-    return (it.flags & 2u) && (unsigned)it.page < (unsigned)kb.num_pages ? ((int64_t)it.page * kb.hkv + it.head) * kb.page_size + it.place : -1;
+  auto slot_of = [&](const Item& it) -> uint32_t { return it.flags & 2u ? kv_slot32(kb, it.page, it.head, it.place) : kNoSlot; };
+  // rows that follow each other (32 tokens inside one page) need one address, others one each
+  struct Rows { uint32_t slot; bool in_line; const uint8_t* at; };
+  auto rows_of = [&](const Item& it) {
+    Rows r;
+    r.slot = slot_of(it);
+    const uint32_t s0 = __shfl_sync(0xffffffffu, r.slot, 0);
+    r.in_line = __all_sync(0xffffffffu, r.slot != kNoSlot && r.slot == s0 + lane);
+    r.at = codes + ((int64_t)s0 + c_tok) * C::RB;
+    return r;
   };
-  auto take = [&](int64_t slot, int piece) {
-    const int64_t s = __shfl_sync(0xffffffffu, slot, c_tok + piece * C::TPI);
-    return s >= 0 ? __ldg(reinterpret_cast<const uint4*>(codes + s * C::RB)) : make_uint4(0, 0, 0, 0);
+  auto take = [&](const Rows& r, int piece) {
+    if (r.in_line) return __ldg(reinterpret_cast<const uint4*>(r.at + piece * (C::TPI * C::RB)));
+    const uint32_t s = __shfl_sync(0xffffffffu, r.slot, c_tok + piece * C::TPI);
+    return s != kNoSlot ? __ldg(reinterpret_cast<const uint4*>(codes + (int64_t)s * C::RB)) : make_uint4(0, 0, 0, 0);
   };
 
   Item nxt = fetch();
   if (!(nxt.flags & 1u)) return;
-  int64_t slot = slot_of(nxt);
+  Rows rows = rows_of(nxt);
   uint32_t flags = nxt.flags;
   nxt = fetch();
   uint4 u[G];
 #pragma unroll
-  for (int i = 0; i < G; ++i) u[i] = take(slot, i);
-  float scale = slot >= 0 ? __ldg(scales + slot) : 0.f;
-  uint32_t zero = FMT == GL_KV_INT4 && slot >= 0 ? __ldg(zeros + slot) : 0u;
+  for (int i = 0; i < G; ++i) u[i] = take(rows, i);
+  float scale = rows.slot != kNoSlot ? __ldg(scales + rows.slot) : 0.f;
+  uint32_t zero = FMT == GL_KV_INT4 && rows.slot != kNoSlot ? __ldg(zeros + rows.slot) : 0u;
 
 #pragma unroll 1
   for (int n = 0; flags & 1u; ++n) {
@@ -213,20 +244,23 @@ __device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh
     const bool apart = (draft && p.mask != nullptr) || (int)(hi >> 23) - (int)(lo >> 23) >= kSpread;
     const int e = apart ? 0 : pow2_above(hi) - kRoom<FMT>;
     const bool number = fabsf(scale) < INFINITY, none = apart && scale < 1e-30f;
-    const uint32_t valid = __ballot_sync(0xffffffffu, slot >= 0);
+    const uint32_t valid = __ballot_sync(0xffffffffu, rows.slot != kNoSlot);
     // Values that are not numbers would reach every row through P V', so V' is 0 there, and the exponent is NaN, which only the
     // rows that see the token meet.  (e4m3's NaN codes matter where some rows do not see the token.)
     uint32_t bad = values ? __ballot_sync(0xffffffffu, !number) : 0u;
     const uint32_t ratio = !number ? (values ? 0u : 0x00007fffu) : values && none ? 0u : apart ? 0x00003c00u : split_half(scale * pow2(-e));
     const uint32_t zz = (0x6400u + zero) * 0x10001u;
-    const int64_t slot_next = slot_of(nxt);
+    const Rows rows_next = rows_of(nxt);
 
     if (n >= 2 && !warp_wait(&empty_bar[st], ((n >> 1) & 1) ^ 1, abort)) return;
     uint8_t* dst = tiles + st * Lay<D>::TILE;
 #pragma unroll 1
     for (int g = 0; g < C::N; g += G) {
       const bool last = g + G >= C::N;                                    // then the pieces of the next tile follow
-      const int64_t from = last ? slot_next : slot;
+      Rows from;
+      from.slot = last ? rows_next.slot : rows.slot;
+      from.in_line = last ? rows_next.in_line : rows.in_line;
+      from.at = last ? rows_next.at : rows.at;
       const int base_piece = last ? 0 : g + G;
 #pragma unroll
       for (int i = 0; i < G; ++i) {
@@ -269,10 +303,10 @@ __device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh
     __syncwarp();
     if (lane == 0) mbar_arrive(&full_bar[st]);
     flags = nxt.flags;
-    slot = slot_next;
+    rows = rows_next;
     if (flags & 1u) {
-      scale = slot >= 0 ? __ldg(scales + slot) : 0.f;
-      if (FMT == GL_KV_INT4) zero = slot >= 0 ? __ldg(zeros + slot) : 0u;
+      scale = rows.slot != kNoSlot ? __ldg(scales + rows.slot) : 0.f;
+      if (FMT == GL_KV_INT4) zero = rows.slot != kNoSlot ? __ldg(zeros + rows.slot) : 0u;
       nxt = fetch();
     }
   }
@@ -437,7 +471,7 @@ __device__ __forceinline__ void stream_role(const KvAttendParams& p, Shared& sh,
             tmem_ld_fence(x);
             float top = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < 32; k += 2) top = fmaxf(top, fmaxf(__uint_as_float(x[k]), __uint_as_float(x[k + 1])));
+            for (int k = 0; k < 32; k += 2) top = max3(top, __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
             t_top = fmaxf(t_top, fmaf(top, qs * meta.ks[h], meta.vs_log2[h]));
           }
         } else {
@@ -476,16 +510,21 @@ __device__ __forceinline__ void stream_role(const KvAttendParams& p, Shared& sh,
             tmem_ld_32x32(ts + 32 * h, x);
             tmem_ld_fence(x);
             const float a = qs * meta.ks[h], sub = meta.vs_log2[h] + to_p;
-            float s0 = 0.f, s1 = 0.f;
+            const uint64_t a2 = pack2(a, a), sub2 = pack2(sub, sub);
+            uint64_t sum2 = 0ull;
             uint32_t pk[16];
 #pragma unroll
             for (int k = 0; k < 32; k += 2) {
-              const float e0 = kv_exp2(fmaf(__uint_as_float(x[k]), a, sub)), e1 = kv_exp2(fmaf(__uint_as_float(x[k + 1]), a, sub));
-              s0 += e0;
-              s1 += e1;
+              float e0, e1;
+              unpack2(fma2(pack2(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), a2, sub2), e0, e1);
+              e0 = kv_exp2(e0);
+              e1 = kv_exp2(e1);
+              sum2 = add2(sum2, pack2(e0, e1));
               const __half2 hh = __floats2half2_rn(e0, e1);
               pk[k >> 1] = *reinterpret_cast<const uint32_t*>(&hh);
             }
+            float s0, s1;
+            unpack2(sum2, s0, s1);
             l = fmaf(s0 + s1, meta.vs_inv[h], l);
             tmem_st_16(ts + h * 16, pk);                              // (columns whose scores have been read)
           }
