@@ -56,18 +56,19 @@ template <int D, int FMT> struct Shape {
   static constexpr int LOOP = kWarps * kStages * STAGE;
 };
 
-template <int D, int FMT, int MT, typename T>
-__global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 3 : 2) kv_attend_mma_kernel(const KvAttendParams p) {
+// Transposed products: S^T = K Q^T and O^T = V^T P^T, so that the tokens (keys) or the channels (values) are the 16 rows of the
+// MMA and 8 query rows its columns: a single token of a group of 8 heads fills them.  NR tiles of 8 query rows.
+template <int D, int FMT, int NR, typename T>
+__global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 3 : 2) kv_attend_mma_kernel(const KvAttendParams p) {
   using S = Shape<D, FMT>;
-  constexpr int RB = S::RB, CPT = RB / 16, NT = D / 8, KS = D / 16, ROWS = 16 * MT;
+  constexpr int RB = S::RB, CPT = RB / 16, NT = D / 8, KS = D / 16, ROWS = 8 * NR;
   constexpr float kShift = 15.f;
   extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ KvPlaceScratch place_scratch;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const KvBatch& kb = p.kb;
   gl_launch_dependents();
   gl_grid_dependency_wait();
-
-  __shared__ KvPlaceScratch place_scratch;
   KvWalk<ROWS> walk;
   walk.start(p, kv_place_of_block<ROWS, kWarps * 32>(p, blockIdx.x, place_scratch), blockIdx.x);
 
@@ -75,76 +76,16 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 3 : 2) kv_attend_mma_ke
   const uint32_t ring_u = smem_addr(ring);
 
   KvPiece pc;
+  KvCut cut{};
   while (walk.next(p, blockIdx.x, pc)) {
+    KvWalk<ROWS>::note(cut, pc);
     const int first = pc.s.first, ctx = pc.s.ctx, rows = pc.rows, kvh = pc.head;
     const int c0 = pc.t0 * kKvTile, c1 = min(pc.t1 * kKvTile, pc.s.len);
     const int64_t pt_row = (int64_t)walk.b * kb.pt_stride;
-
-    // ---- queries as the A operand, channels in the order in which the codes come out of their words
-    uint32_t qa[MT][KS][4];
-    float qs[MT][2];
-    int q_tok[MT][2];                                     // which new token the row belongs to
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const bool live = m * 16 + g + hf * 8 < rows;
-        const int r = pc.row0 + (live ? m * 16 + g + hf * 8 : 0), t = r / p.group, head = kvh * p.group + (r - t * p.group);
-        q_tok[m][hf] = t;
-        const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)(first + t) * p.q_sn + (int64_t)head * p.q_sh;
-        uint32_t w[D / 8];                                // this lane's D / 4 channels
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          // 8-bit rows: chunks c and c + 4 of 16 channels; 4-bit rows: one piece of D / 4 channels
-          const int at = FMT == GL_KV_INT4 ? c * (D / 4) + i * 8 : (i >> 1) * 64 + c * 16 + (i & 1) * 8;
-          uint4 u = make_uint4(0, 0, 0, 0);
-          if (live) u = *reinterpret_cast<const uint4*>(src + at);
-          w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
-        }
-        float factor = 1.f;
-        if constexpr (sizeof(T) == 2 && !IsHalf<T>::value) {
-          uint32_t top = 0;
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
-          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          const int ex = min(max((int)(top >> 7), 1), 253);
-          const float inv = __int_as_float((254 - ex) << 23);
-          factor = __int_as_float(ex << 23);
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
-            const __half2 h = __floats2half2_rn(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xffff0000u) * inv);
-            w[i] = *reinterpret_cast<const uint32_t*>(&h);
-          }
-        }
-        qs[m][hf] = p.scale_log2 * factor;
-#pragma unroll
-        for (int j = 0; j < KS; ++j) {
-          if (FMT == GL_KV_INT4) {
-            const int i4 = (j >> 1) * 4;                  // words of channels 8 (j / 2) ..: (0,1) (2,3) (4,5) (6,7)
-            qa[m][j][hf] = prmt(w[i4 + (j & 1)], w[i4 + 2 + (j & 1)], 0x5410);
-            qa[m][j][2 + hf] = prmt(w[i4 + (j & 1)], w[i4 + 2 + (j & 1)], 0x7632);
-          } else {
-            qa[m][j][hf] = w[2 * j];
-            qa[m][j][2 + hf] = w[2 * j + 1];
-          }
-        }
-      }
-
-    float o[MT][NT][4], mx[MT][2], sum[MT][2];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[m][i][e] = 0.f;
-      mx[m][0] = mx[m][1] = -INFINITY;
-      sum[m][0] = sum[m][1] = 0.f;
-    }
-
     const int tiles = c1 > c0 ? (c1 - c0 + kTile - 1) / kTile : 0;
     const int mine = (tiles - warp + kWarps - 1) / kWarps;              // tiles warp, warp + 4, ..
 
+    // ---- tokens of a tile into shared memory, kStages - 1 tiles ahead
     auto slot_of = [&](int i) -> uint32_t {                             // lane's token of the warp's i-th tile
       const int pos = c0 + (warp + i * kWarps) * kTile + lane;
       if (i >= mine || pos >= c1) return kNoSlot;
@@ -202,6 +143,68 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 3 : 2) kv_attend_mma_ke
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) issue(i);
 
+    // ---- queries as the B operand (column = row g of a tile of 8), channels in the order in which codes come out of their words
+    uint32_t qb[NR][KS][2];
+    float qs[NR][2];                                      // log2(e) * scale * power of two, of rows 2c and 2c + 1
+    int q_tok[NR][2];                                     // their tokens
+#pragma unroll
+    for (int m = 0; m < NR; ++m) {
+      const bool live = m * 8 + g < rows;
+      const int r = pc.row0 + (live ? m * 8 + g : 0), t = r / p.group, head = kvh * p.group + (r - t * p.group);
+      const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)(first + t) * p.q_sn + (int64_t)head * p.q_sh;
+      uint32_t w[D / 8];                                  // this lane's D / 4 channels
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        // 8-bit rows: chunks c and c + 4 of 16 channels; 4-bit rows: one piece of D / 4 channels
+        const int at = FMT == GL_KV_INT4 ? c * (D / 4) + i * 8 : (i >> 1) * 64 + c * 16 + (i & 1) * 8;
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (live) u = *reinterpret_cast<const uint4*>(src + at);
+        w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+      }
+      float factor = 1.f;
+      if constexpr (!IsHalf<T>::value) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int ex = min(max((int)(top >> 7), 1), 253);
+        const float inv = __int_as_float((254 - ex) << 23);
+        factor = __int_as_float(ex << 23);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) w[i] = kv_pair<__half>(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xffff0000u) * inv);
+      }
+      const float f = p.scale_log2 * factor;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {                       // row 2c + e is column g = 2c + e of lanes 4 g ..
+        qs[m][e] = __shfl_sync(0xffffffffu, f, (2 * c + e) * 4);
+        q_tok[m][e] = __shfl_sync(0xffffffffu, t, (2 * c + e) * 4);
+      }
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        if (FMT == GL_KV_INT4) {
+          const int i4 = (j >> 1) * 4;                    // words of channels 8 (j / 2) ..: (0,1) (2,3) (4,5) (6,7)
+          qb[m][j][0] = prmt(w[i4 + (j & 1)], w[i4 + 2 + (j & 1)], 0x5410);
+          qb[m][j][1] = prmt(w[i4 + (j & 1)], w[i4 + 2 + (j & 1)], 0x7632);
+        } else {
+          qb[m][j][0] = w[2 * j];
+          qb[m][j][1] = w[2 * j + 1];
+        }
+      }
+    }
+
+    float o[NR][NT / 2][4], mx[NR][2], sum[NR][2];
+#pragma unroll
+    for (int m = 0; m < NR; ++m) {
+#pragma unroll
+      for (int i = 0; i < NT / 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[m][i][e] = 0.f;
+      mx[m][0] = mx[m][1] = -INFINITY;
+      sum[m][0] = sum[m][1] = 0.f;
+    }
+
+#pragma unroll 1
     for (int i = 0; i < mine; ++i) {
       issue(i + kStages - 1);
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
@@ -236,155 +239,154 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 3 : 2) kv_attend_mma_ke
       *reinterpret_cast<float*>(st + S::RV_AT + lane * 4) = __frcp_rn(vs_lane);
       __syncwarp();
 
-      // ---- scores
-      float s[MT][4][4];
+      // ---- scores of 2 x 16 tokens: this lane's are tokens g and g + 8, rows 2c and 2c + 1
+      float s[NR][2][4];
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
+      for (int h = 0; h < 2; ++h) {
+        uint32_t kw[2][RB / 16], zk[2];
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[m][nt][e] = 0.f;
-        const int t = nt * 8 + g;
-        uint32_t kw[RB / 16];
-        if constexpr (RB == 128) {
-          *reinterpret_cast<uint4*>(kw) = *reinterpret_cast<const uint4*>(st + S::K_AT + k_place<RB>(t, c));
-          *reinterpret_cast<uint4*>(kw + 4) = *reinterpret_cast<const uint4*>(st + S::K_AT + k_place<RB>(t, c + 4));
-        } else if constexpr (RB == 64) {
-          *reinterpret_cast<uint4*>(kw) = *reinterpret_cast<const uint4*>(st + S::K_AT + k_place<RB>(t, c));
-        } else {
-          *reinterpret_cast<uint2*>(kw) = *reinterpret_cast<const uint2*>(st + S::K_AT + t * RB + c * 8);
+        for (int y = 0; y < 2; ++y) {
+          const int t = h * 16 + y * 8 + g;
+          if constexpr (RB == 128) {
+            *reinterpret_cast<uint4*>(kw[y]) = *reinterpret_cast<const uint4*>(st + S::K_AT + k_place<RB>(t, c));
+            *reinterpret_cast<uint4*>(kw[y] + 4) = *reinterpret_cast<const uint4*>(st + S::K_AT + k_place<RB>(t, c + 4));
+          } else if constexpr (RB == 64) {
+            *reinterpret_cast<uint4*>(kw[y]) = *reinterpret_cast<const uint4*>(st + S::K_AT + k_place<RB>(t, c));
+          } else {
+            *reinterpret_cast<uint2*>(kw[y]) = *reinterpret_cast<const uint2*>(st + S::K_AT + t * RB + c * 8);
+          }
+          zk[y] = 0;
+          if (FMT == GL_KV_INT4) zk[y] = (0x6400u + st[S::KZ_AT + t]) * 0x10001u;
         }
-        uint32_t zk = 0;
-        if (FMT == GL_KV_INT4) {
-          zk = 0x6400u + st[S::KZ_AT + t];
-          zk |= zk << 16;
-        }
+#pragma unroll
+        for (int m = 0; m < NR; ++m)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[m][h][e] = 0.f;
 #pragma unroll
         for (int j = 0; j < KS; ++j) {
-          uint32_t b0, b1;
+          uint32_t a[4];
           if (FMT == GL_KV_INT4) {
-            const uint32_t w = kw[j >> 1] >> ((j & 1) * 8);
-            b0 = kv_nibbles(w, zk);
-            b1 = kv_nibbles(w >> 4, zk);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const uint32_t w = kw[y][j >> 1] >> ((j & 1) * 8);
+              a[y] = kv_nibbles(w, zk[y]);
+              a[2 + y] = kv_nibbles(w >> 4, zk[y]);
+            }
           } else {
-            kv_bytes<FMT>(kw[j], b0, b1);
+            kv_bytes<FMT>(kw[0][j], a[0], a[2]);
+            kv_bytes<FMT>(kw[1][j], a[1], a[3]);
           }
 #pragma unroll
-          for (int m = 0; m < MT; ++m) mma16816(s[m][nt], qa[m][j], b0, b1);
+          for (int m = 0; m < NR; ++m) mma16816(s[m][h], a, qb[m][j][0], qb[m][j][1]);
         }
       }
 
       // ---- exponents
+      float rv[2][2];
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
-        const float2 ks = *reinterpret_cast<const float2*>(st + S::KS_AT + (nt * 8 + 2 * c) * 4);
-        const float2 lv = *reinterpret_cast<const float2*>(st + S::VS_AT + (nt * 8 + 2 * c) * 4);
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          s[m][nt][0] = fmaf(s[m][nt][0] * ks.x, qs[m][0], lv.x);
-          s[m][nt][1] = fmaf(s[m][nt][1] * ks.y, qs[m][0], lv.y);
-          s[m][nt][2] = fmaf(s[m][nt][2] * ks.x, qs[m][1], lv.x);
-          s[m][nt][3] = fmaf(s[m][nt][3] * ks.y, qs[m][1], lv.y);
+        for (int y = 0; y < 2; ++y) {
+          const int t = h * 16 + y * 8 + g;
+          const float ks = *reinterpret_cast<const float*>(st + S::KS_AT + t * 4), lv = *reinterpret_cast<const float*>(st + S::VS_AT + t * 4);
+          rv[h][y] = *reinterpret_cast<const float*>(st + S::RV_AT + t * 4);
+#pragma unroll
+          for (int m = 0; m < NR; ++m)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) s[m][h][2 * y + e] = fmaf(s[m][h][2 * y + e] * ks, qs[m][e], lv);
         }
-      }
       if (!whole) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int m = 0; m < NR; ++m)
 #pragma unroll
-          for (int nt = 0; nt < 4; ++nt)
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int t = nt * 8 + 2 * c + (e & 1), at = tile0 + t - ctx;     // >= 0: which new token
+              const int t = h * 16 + (e >> 1) * 8 + g, at = tile0 + t - ctx;     // >= 0: which new token
               bool sees = (there >> t) & 1u;
               if (at >= 0) {
-                const int own = q_tok[m][e >> 1];
+                const int own = q_tok[m][e & 1];
                 sees = sees && (p.mask == nullptr ? at <= own : at < p.mask_cols && p.mask[(int64_t)(first + own) * p.mask_stride + at] != 0);
               }
-              if (!sees) s[m][nt][e] = -INFINITY;
+              if (!sees) s[m][h][e] = -INFINITY;
             }
       }
-      uint32_t pa[MT][2][4];
+      uint32_t pb[NR][2][2];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        float top[2] = {mx[m][0], mx[m][1]};
+      for (int m = 0; m < NR; ++m) {
+        float top[2];
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-          top[0] = fmaxf(top[0], fmaxf(s[m][nt][0], s[m][nt][1]));
-          top[1] = fmaxf(top[1], fmaxf(s[m][nt][2], s[m][nt][3]));
-        }
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          top[hf] = fmaxf(top[hf], __shfl_xor_sync(0xffffffffu, top[hf], 1));
-          top[hf] = fmaxf(top[hf], __shfl_xor_sync(0xffffffffu, top[hf], 2));
+        for (int e = 0; e < 2; ++e) {
+          top[e] = fmaxf(fmaxf(s[m][0][e], s[m][0][2 + e]), fmaxf(s[m][1][e], s[m][1][2 + e]));
+          top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 4));
+          top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 8));
+          top[e] = fmaxf(fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 16)), mx[m][e]);
         }
         if (__any_sync(0xffffffffu, top[0] > mx[m][0] || top[1] > mx[m][1])) {
           const float f0 = mx[m][0] == top[0] ? 1.f : kv_exp2(mx[m][0] - top[0]), f1 = mx[m][1] == top[1] ? 1.f : kv_exp2(mx[m][1] - top[1]);
           sum[m][0] *= f0;
           sum[m][1] *= f1;
 #pragma unroll
-          for (int n = 0; n < NT; ++n) { o[m][n][0] *= f0; o[m][n][1] *= f0; o[m][n][2] *= f1; o[m][n][3] *= f1; }
+          for (int n = 0; n < NT / 2; ++n) { o[m][n][0] *= f0; o[m][n][1] *= f1; o[m][n][2] *= f0; o[m][n][3] *= f1; }
           mx[m][0] = top[0];
           mx[m][1] = top[1];
         }
-        const float sub0 = top[0] == -INFINITY ? 0.f : top[0] - kShift, sub1 = top[1] == -INFINITY ? 0.f : top[1] - kShift;
+        const float sub[2] = {top[0] == -INFINITY ? 0.f : top[0] - kShift, top[1] == -INFINITY ? 0.f : top[1] - kShift};
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-          const float2 rv = *reinterpret_cast<const float2*>(st + S::RV_AT + (nt * 8 + 2 * c) * 4);
-          const float e0 = kv_exp2(s[m][nt][0] - sub0), e1 = kv_exp2(s[m][nt][1] - sub0), e2 = kv_exp2(s[m][nt][2] - sub1), e3 = kv_exp2(s[m][nt][3] - sub1);
-          if (whole) {
-            sum[m][0] = fmaf(e0, rv.x, fmaf(e1, rv.y, sum[m][0]));
-            sum[m][1] = fmaf(e2, rv.x, fmaf(e3, rv.y, sum[m][1]));
-          } else {                                         // a token that is not seen has the weight 0, also where its scale is NaN
-            sum[m][0] += (s[m][nt][0] != -INFINITY ? e0 * rv.x : 0.f) + (s[m][nt][1] != -INFINITY ? e1 * rv.y : 0.f);
-            sum[m][1] += (s[m][nt][2] != -INFINITY ? e2 * rv.x : 0.f) + (s[m][nt][3] != -INFINITY ? e3 * rv.y : 0.f);
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const float s0 = s[m][h][2 * y], s1 = s[m][h][2 * y + 1], e0 = kv_exp2(s0 - sub[0]), e1 = kv_exp2(s1 - sub[1]);
+            if (whole) {
+              sum[m][0] = fmaf(e0, rv[h][y], sum[m][0]);
+              sum[m][1] = fmaf(e1, rv[h][y], sum[m][1]);
+            } else {                                       // a token that is not seen has the weight 0, also where its scale is NaN
+              sum[m][0] += s0 != -INFINITY ? e0 * rv[h][y] : 0.f;
+              sum[m][1] += s1 != -INFINITY ? e1 * rv[h][y] : 0.f;
+            }
+            // (token g, rows 2c, 2c + 1) -> (tokens 2c, 2c + 1, row g): the B operand of the second product
+            asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[m][h][y]) : "r"(kv_pair<__half>(e0, e1)));
           }
-          const __half2 lo = __floats2half2_rn(e0, e1), hi = __floats2half2_rn(e2, e3);
-          pa[m][nt >> 1][(nt & 1) * 2] = *reinterpret_cast<const uint32_t*>(&lo);
-          pa[m][nt >> 1][(nt & 1) * 2 + 1] = *reinterpret_cast<const uint32_t*>(&hi);
-        }
       }
 
-      // ---- weighted codes: column n of the B operand's tile i is channel NT n + i
+      // ---- weighted codes: rows g and g + 8 of the A operand's tile i are channels NT g + 2 i and NT g + 2 i + 1
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
+      for (int h = 0; h < 2; ++h) {
         constexpr int VW = RB / 32;                        // words of a token's row that this lane takes
         uint32_t vw[4][VW];
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
-          const int t = kk * 16 + 2 * c + (q4 & 1) + (q4 >> 1) * 8;
+          const int t = h * 16 + 2 * c + (q4 & 1) + (q4 >> 1) * 8;
           if constexpr (RB == 128) *reinterpret_cast<uint4*>(vw[q4]) = *reinterpret_cast<const uint4*>(st + S::V_AT + v_place<RB>(t, g));
           else if constexpr (RB == 64) *reinterpret_cast<uint2*>(vw[q4]) = *reinterpret_cast<const uint2*>(st + S::V_AT + v_place<RB>(t, g >> 1) + (g & 1) * 8);
           else vw[q4][0] = *reinterpret_cast<const uint32_t*>(st + S::V_AT + v_place<RB>(t, g >> 2) + (g & 3) * 4);
         }
         uint32_t z0 = 0, z1 = 0;
         if (FMT == GL_KV_INT4) {
-          const uint8_t* z = st + S::VZ_AT + kk * 16 + 2 * c;
+          const uint8_t* z = st + S::VZ_AT + h * 16 + 2 * c;
           z0 = (0x6400u + z[0]) | (0x6400u + z[1]) << 16;
           z1 = (0x6400u + z[8]) | (0x6400u + z[9]) << 16;
         }
 #pragma unroll
-        for (int w = 0; w < VW; ++w) {
+        for (int w = 0; w < VW; ++w)
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
             if (FMT == GL_KV_INT4) {
               const uint32_t x = prmt(vw[0][w], vw[1][w], hf ? 0x7632 : 0x5410), y = prmt(vw[2][w], vw[3][w], hf ? 0x7632 : 0x5410);
 #pragma unroll
-              for (int n = 0; n < 4; ++n) {
-                const uint32_t b0 = kv_nibbles(x >> (4 * n), z0), b1 = kv_nibbles(y >> (4 * n), z1);
+              for (int n = 0; n < 2; ++n) {
+                const uint32_t a[4] = {kv_nibbles(x >> (8 * n), z0), kv_nibbles(x >> (8 * n + 4), z0), kv_nibbles(y >> (8 * n), z1), kv_nibbles(y >> (8 * n + 4), z1)};
 #pragma unroll
-                for (int m = 0; m < MT; ++m) mma16816(o[m][8 * w + 4 * hf + n], pa[m][kk], b0, b1);
+                for (int m = 0; m < NR; ++m) mma16816(o[m][4 * w + 2 * hf + n], a, pb[m][h][0], pb[m][h][1]);
               }
             } else {
-              uint32_t b0[2], b1[2];
-              kv_bytes<FMT>(prmt(vw[0][w], vw[1][w], hf ? 0x7362 : 0x5140), b0[0], b0[1]);
-              kv_bytes<FMT>(prmt(vw[2][w], vw[3][w], hf ? 0x7362 : 0x5140), b1[0], b1[1]);
+              uint32_t a[4];
+              kv_bytes<FMT>(prmt(vw[0][w], vw[1][w], hf ? 0x7362 : 0x5140), a[0], a[1]);
+              kv_bytes<FMT>(prmt(vw[2][w], vw[3][w], hf ? 0x7362 : 0x5140), a[2], a[3]);
 #pragma unroll
-              for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int m = 0; m < MT; ++m) mma16816(o[m][4 * w + 2 * hf + n], pa[m][kk], b0[n], b1[n]);
+              for (int m = 0; m < NR; ++m) mma16816(o[m][2 * w + hf], a, pb[m][h][0], pb[m][h][1]);
             }
           }
-        }
       }
       __syncwarp();                                        // the stage may be overwritten
     }
@@ -392,41 +394,39 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 3 : 2) kv_attend_mma_ke
     // ---- the warps' parts become one: each scales its own to the common maximum
     asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < NR; ++m)
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        sum[m][hf] += __shfl_xor_sync(0xffffffffu, sum[m][hf], 1);
-        sum[m][hf] += __shfl_xor_sync(0xffffffffu, sum[m][hf], 2);
+      for (int e = 0; e < 2; ++e) {
+        sum[m][e] += __shfl_xor_sync(0xffffffffu, sum[m][e], 4);
+        sum[m][e] += __shfl_xor_sync(0xffffffffu, sum[m][e], 8);
+        sum[m][e] += __shfl_xor_sync(0xffffffffu, sum[m][e], 16);
       }
     __syncthreads();                                       // every warp is through with its ring
     float* part = reinterpret_cast<float*>(smem);          // [warps][ROWS][D]
     float2* ml = reinterpret_cast<float2*>(part + kWarps * ROWS * D);    // [warps][ROWS]
-    if (c == 0)
+    if (g == 0)
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int m = 0; m < NR; ++m)
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) ml[warp * ROWS + m * 16 + g + hf * 8] = make_float2(mx[m][hf], sum[m][hf]);
+        for (int e = 0; e < 2; ++e) ml[warp * ROWS + m * 8 + 2 * c + e] = make_float2(mx[m][e], sum[m][e]);
     __syncthreads();
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < NR; ++m)
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int r = m * 16 + g + hf * 8;
+      for (int e = 0; e < 2; ++e) {
+        const int r = m * 8 + 2 * c + e;
         float top = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[w * ROWS + r].x);
-        const float f = mx[m][hf] == -INFINITY ? 0.f : kv_exp2(mx[m][hf] - top);
-        float* dst = part + (warp * ROWS + r) * D + 2 * c * NT;
+        const float f = mx[m][e] == -INFINITY ? 0.f : kv_exp2(mx[m][e] - top);
+        float* dst = part + (warp * ROWS + r) * D + NT * g;
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int i = 0; i < NT; i += 4)
-            *reinterpret_cast<float4*>(dst + e * NT + i) = make_float4(o[m][i][2 * hf + e] * f, o[m][i + 1][2 * hf + e] * f, o[m][i + 2][2 * hf + e] * f, o[m][i + 3][2 * hf + e] * f);
+        for (int i = 0; i < NT / 2; i += 2)
+          *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(o[m][i][e] * f, o[m][i][2 + e] * f, o[m][i + 1][e] * f, o[m][i + 1][2 + e] * f);
       }
     __syncthreads();
-    for (int at = tid * 4; at < ROWS * D; at += kWarps * 32 * 4) {
+    for (int at = tid * 4; at < rows * D; at += kWarps * 32 * 4) {
       const int r = at / D, d = at % D;
-      if (r >= rows) break;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
       float top = -INFINITY, l = 0.f;
 #pragma unroll
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 3 : 2) kv_attend_mma_ke
         const float4 x = *reinterpret_cast<const float4*>(part + (w * ROWS + r) * D + d);
         acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
         const float2 m2 = ml[w * ROWS + r];
-        l += m2.x == -INFINITY ? 0.f : m2.y * kv_exp2(m2.x - top);
+        l += m2.x == -INFINITY ? (m2.y == 0.f ? 0.f : m2.y) : m2.y * kv_exp2(m2.x - top);
       }
       const int rr = pc.row0 + r, t = rr / p.group;
       if (pc.whole) {
@@ -449,144 +449,170 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 3 : 2) kv_attend_mma_ke
     }
     __syncthreads();
   }
+  if (tid == 0 && p.cuts != nullptr) p.cuts[blockIdx.x] = cut;
 }
 
-// Joins the parts of the units that block borders cut.  Blocks (i, *) look after border i + 1 if it is the first one in its
-// unit.  Few parts (a border or two in a unit): a warp per row; many (one long sequence): a block per row, warp w takes parts
-// w, w + 8, ..
+// Joins the parts of the units that block borders cut: blocks (i, *) look after the unit that block i began and did not
+// finish.  Few parts: a warp per row, 8 rows at a time; many (one long sequence): a block per row, warp w takes parts w, w + 8, ..
+constexpr int kJoinMax = 1024;                 // thread blocks of a launch, at most
 template <int ROWS, int D, typename T>
 __global__ void __launch_bounds__(256) kv_attend_join_kernel(const KvAttendParams p) {
-  __shared__ KvPlaceScratch place_scratch;
   __shared__ float4 acc_s[8][D / 4];
   __shared__ float2 red[8];
+  __shared__ float weight[kJoinMax];
+  __shared__ int last;
   constexpr int V = D / 32;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, border = blockIdx.x + 1;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, i0 = blockIdx.x;
   gl_launch_dependents();
   gl_grid_dependency_wait();
-  const KvPlace pl = kv_place_of_block<ROWS, 256>(p, border, place_scratch);
-  if (pl.b < 0) return;
-  const KvSeq s = kv_seq<ROWS>(p, pl.b);
-  const int u = (int)kv_div(pl.off, s.tiles);
-  const int64_t begin = pl.prefix + (int64_t)u * s.tiles;
-  if (begin == pl.prefix + pl.off) return;                       // the border is the unit's own
-  const KvShare share(pl.total, p.blocks);
-  const int i0 = share.owner(begin), i1 = share.owner(begin + s.tiles - 1);      // every block from i0 to i1 has tiles of the unit
-  if (i0 != border - 1) return;                                  // an earlier border of the unit does the work
-  const int head = u / s.blocks, row0 = kv_row_block(u - head * s.blocks, s.blocks) * ROWS, rows = min(ROWS, s.new_b * p.group - row0);
-  auto part = [&](int i) { return (int64_t)(2 * i + (i == i0 ? 1 : 0)) * ROWS; };
-  const bool few = i1 - i0 < 16;
-  const int first = few ? i0 : i0 + warp, step = few ? 1 : 8;
+  const KvCut cut = p.cuts[i0];
+  if ((cut.flags & 1) == 0) return;
+  // the unit's last part: the first later block that finishes what it goes on with (blocks in between hold nothing else)
+  if (tid == 0) last = p.blocks - 1;
+  __syncthreads();
+  for (int i = i0 + 1 + tid; i < p.blocks; i += 256) {
+    if (i > *(volatile int*)&last) break;
+    if (p.cuts[i].flags & 4) { atomicMin(&last, i); break; }
+  }
+  __syncthreads();
+  const int i1 = last, n = i1 - i0 + 1;
+  auto part = [&](int k) { return (int64_t)(k == 0 ? 2 * i0 + 1 : 2 * (i0 + k)) * ROWS; };
+  auto dst_of = [&](int r) {
+    const int rr = cut.row0 + r, t = rr / p.group;
+    return reinterpret_cast<T*>(p.out) + ((int64_t)(cut.first + t) * p.hq + cut.head * p.group + (rr - t * p.group)) * D;
+  };
+  // weight of a part: 0 where it saw nothing; a sum of NaN with the maximum -inf stays one
+  auto weight_of = [&](float2 ml, float top) { return ml.y == 0.f ? 0.f : ml.x == -INFINITY ? ml.y : kv_exp2(ml.x - top); };
 
-  for (int r = few ? blockIdx.y * 8 + warp : blockIdx.y; r < rows; r += gridDim.y * (few ? 8 : 1)) {
-    // maximum of the parts that saw anything (a sum of NaN counts)
+  if (n <= 16) {
+    for (int r = blockIdx.y * 8 + warp; r < cut.rows; r += gridDim.y * 8) {
+      const float2 ml = lane < n ? p.part_ml[part(lane) + r] : make_float2(-INFINITY, 0.f);
+      float top = ml.y != 0.f ? ml.x : -INFINITY;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float f = weight_of(ml, top);
+      float l = f == 0.f ? 0.f : ml.y * f;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      float acc[V] = {};
+#pragma unroll 4
+      for (int k = 0; k < n; ++k) {
+        float x[V];
+        kv_load_n<V>(p.part_o + (part(k) + r) * D + lane * V, x);
+        const float w = __shfl_sync(0xffffffffu, f, k);
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[j] += w == 0.f ? 0.f : x[j] * w;
+      }
+      const float q = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] = l == 0.f ? 0.f : acc[j] * q;
+      kv_store_n<T, V>(dst_of(r) + lane * V, acc);
+    }
+    return;
+  }
+  for (int r = blockIdx.y; r < cut.rows; r += gridDim.y) {
     float top = -INFINITY;
-    for (int i = few ? i0 + lane : i0 + tid; i <= i1; i += few ? 32 : 256) {
-      const float2 ml = p.part_ml[part(i) + r];
+    for (int k = tid; k < n; k += 256) {
+      const float2 ml = p.part_ml[part(k) + r];
       if (ml.y != 0.f) top = fmaxf(top, ml.x);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (!few) {
-      if (lane == 0) red[warp].x = top;
-      __syncthreads();
+    if (lane == 0) red[warp].x = top;
+    __syncthreads();
 #pragma unroll
-      for (int w = 0; w < 8; ++w) top = fmaxf(top, red[w].x);
-    }
-    float acc[V] = {};
+    for (int w = 0; w < 8; ++w) top = fmaxf(top, red[w].x);
     float l = 0.f;
-#pragma unroll 4
-    for (int i = first; i <= i1; i += step) {
-      const float2 ml = p.part_ml[part(i) + r];
-      const float f = ml.y == 0.f ? 0.f : ml.x == -INFINITY ? ml.y : kv_exp2(ml.x - top);    // -inf with a sum: the sum is NaN
+    for (int k = tid; k < n; k += 256) {
+      const float2 ml = p.part_ml[part(k) + r];
+      const float f = weight_of(ml, top);
+      weight[k] = f;
+      l += f == 0.f ? 0.f : ml.y * f;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (lane == 0) red[warp].y = l;
+    __syncthreads();
+    float acc[V] = {};
+#pragma unroll 8
+    for (int k = warp; k < n; k += 8) {
       float x[V];
-      if constexpr (V == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p.part_o + (part(i) + r) * D + lane * V);
-      else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(p.part_o + (part(i) + r) * D + lane * V);
-      l += ml.y * f;
+      kv_load_n<V>(p.part_o + (part(k) + r) * D + lane * V, x);
+      const float w = weight[k];
 #pragma unroll
-      for (int j = 0; j < V; ++j) acc[j] += ml.y == 0.f ? 0.f : x[j] * f;
+      for (int j = 0; j < V; ++j) acc[j] += w == 0.f ? 0.f : x[j] * w;
     }
-    const int rr = row0 + r, t = rr / p.group;
-    T* dst = reinterpret_cast<T*>(p.out) + ((int64_t)(s.first + t) * p.hq + head * p.group + (rr - t * p.group)) * D;
-    if (!few) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) reinterpret_cast<float*>(acc_s[warp])[lane * V + j] = acc[j];
-      __syncthreads();                                           // (everybody has read the maxima)
-      if (lane == 0) red[warp].y = l;
-      __syncthreads();
-      if (tid < D / 4) {
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        l = 0.f;
+    for (int j = 0; j < V; ++j) reinterpret_cast<float*>(acc_s[warp])[lane * V + j] = acc[j];
+    __syncthreads();
+    if (tid < D / 4) {
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+      l = 0.f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) {
-          const float4 x = acc_s[w][tid];
-          a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
-          l += red[w].y;
-        }
-        kv_store4<T>(dst + tid * 4, a, l);
+      for (int w = 0; w < 8; ++w) {
+        const float4 x = acc_s[w][tid];
+        a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+        l += red[w].y;
       }
-      __syncthreads();
-    } else {
-      const float q = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-      for (int j = 0; j < V; ++j) acc[j] = l == 0.f ? 0.f : acc[j] * q;
-      kv_store_n<T, V>(dst + lane * V, acc);
+      kv_store4<T>(dst_of(r) + tid * 4, a, l);
     }
+    __syncthreads();
   }
 }
 
-template <int D, int FMT, int MT, typename T>
+template <int D, int FMT, int NR, typename T>
 int launch_mma(const KvAttendParams& p, cudaStream_t st) {
-  constexpr int LOOP = Shape<D, FMT>::LOOP, JOIN = kWarps * 16 * MT * (D * 4 + 8), SMEM = LOOP > JOIN ? LOOP : JOIN;
-  if (int rc = kv_allow_smem((const void*)kv_attend_mma_kernel<D, FMT, MT, T>, SMEM)) return rc;
-  GL_CUDA_CHECK(gl_launch_pdl(kv_attend_mma_kernel<D, FMT, MT, T>, dim3((unsigned)p.blocks), dim3(kWarps * 32), SMEM, st, p));
+  constexpr int LOOP = Shape<D, FMT>::LOOP, JOIN = kWarps * 8 * NR * (D * 4 + 8), SMEM = LOOP > JOIN ? LOOP : JOIN;
+  if (int rc = kv_allow_smem((const void*)kv_attend_mma_kernel<D, FMT, NR, T>, SMEM)) return rc;
+  GL_CUDA_CHECK(gl_launch_pdl(kv_attend_mma_kernel<D, FMT, NR, T>, dim3((unsigned)p.blocks), dim3(kWarps * 32), SMEM, st, p));
   return GL_OK;
 }
-template <int D, int FMT, typename T>
-int launch_rows(const KvAttendParams& p, int mt, cudaStream_t st) {
-  return mt == 1 ? launch_mma<D, FMT, 1, T>(p, st) : launch_mma<D, FMT, 2, T>(p, st);
-}
 template <int D, typename T>
-int launch_fmt(const KvAttendParams& p, int fmt, int mt, cudaStream_t st) {
+int launch_fmt(const KvAttendParams& p, int fmt, int rows, cudaStream_t st) {
   switch (fmt) {
-    case GL_KV_FP8: return launch_rows<D, GL_KV_FP8, T>(p, mt, st);
-    case GL_KV_INT8: return launch_rows<D, GL_KV_INT8, T>(p, mt, st);
-    default: return launch_rows<D, GL_KV_INT4, T>(p, mt, st);
+    case GL_KV_FP8: return rows == 8 ? launch_mma<D, GL_KV_FP8, 1, T>(p, st) : launch_mma<D, GL_KV_FP8, 2, T>(p, st);
+    case GL_KV_INT8: return rows == 8 ? launch_mma<D, GL_KV_INT8, 1, T>(p, st) : launch_mma<D, GL_KV_INT8, 2, T>(p, st);
+    default: return rows == 8 ? launch_mma<D, GL_KV_INT4, 1, T>(p, st) : launch_mma<D, GL_KV_INT4, 2, T>(p, st);
   }
 }
 template <int ROWS, int D, typename T>
-int launch_join(const KvAttendParams& p, int live_rows, cudaStream_t st) {
-  const int y = live_rows < 16 ? live_rows : 16;
-  GL_CUDA_CHECK(gl_launch_pdl(kv_attend_join_kernel<ROWS, D, T>, dim3((unsigned)(p.blocks - 1), (unsigned)y), dim3(256), 0, st, p));
+int launch_join(const KvAttendParams& p, int grid_y, cudaStream_t st) {
+  GL_CUDA_CHECK(gl_launch_pdl(kv_attend_join_kernel<ROWS, D, T>, dim3((unsigned)(p.blocks - 1), (unsigned)grid_y), dim3(256), 0, st, p));
   return GL_OK;
-}
-template <int D, typename T>
-int launch_all(const KvAttendParams& p, const gl_kv_args* a, int rows, int live_rows, cudaStream_t st) {
-  if (int rc = rows == kKvTcRows ? gl_kv_attend_tc_launch(p, D, a->format, a->x_dtype, st) : launch_fmt<D, T>(p, a->format, rows / 16, st)) return rc;
-  if (p.blocks == 1) return GL_OK;
-  if (rows == kKvTcRows) return launch_join<kKvTcRows, D, T>(p, live_rows, st);
-  return rows == 16 ? launch_join<16, D, T>(p, live_rows, st) : launch_join<32, D, T>(p, live_rows, st);
 }
 
 struct Plan {
-  int rows, live_rows, blocks;      // rows of a unit, the most of them that are live, thread blocks
+  int rows, blocks, join_y;      // rows of a unit, thread blocks of the main kernel, blocks per cut unit of the join
 };
 
-// Few rows per kv head: the mma.sync kernel, which holds 16 or 32 rows in registers (two blocks per SM); more: the tcgen05
-// kernel with 256 (one per SM).
+template <int D, typename T>
+int launch_all(const KvAttendParams& p, const gl_kv_args* a, const Plan& pl, cudaStream_t st) {
+  if (int rc = pl.rows == kKvTcRows ? gl_kv_attend_tc_launch(p, D, a->format, a->x_dtype, st) : launch_fmt<D, T>(p, a->format, pl.rows, st)) return rc;
+  if (p.blocks == 1) return GL_OK;
+  if (pl.rows == kKvTcRows) return launch_join<kKvTcRows, D, T>(p, pl.join_y, st);
+  return pl.rows == 8 ? launch_join<8, D, T>(p, pl.join_y, st) : launch_join<16, D, T>(p, pl.join_y, st);
+}
+
+// Few rows per kv head: the mma.sync kernel, which holds 8 or 16 rows in registers (three or two blocks per SM); more: the
+// tcgen05 kernel with 256 (one per SM).
 Plan plan_of(const gl_kv_args* a) {
   Plan pl;
   const int group = a->n_q_heads / a->n_kv_heads;
   int64_t max_rows = (int64_t)(a->max_new < a->n_tokens ? a->max_new : a->n_tokens) * group;
   if (max_rows < 1) max_rows = 1;
-  const bool tc = a->kernel_override == 2 || (a->kernel_override == 0 && max_rows > 32);
-  pl.rows = tc ? kKvTcRows : max_rows <= 16 ? 16 : 32;
-  pl.live_rows = (int)(max_rows < pl.rows ? max_rows : pl.rows);
+  const bool tc = a->kernel_override == 2 || (a->kernel_override == 0 && max_rows > 16);
+  pl.rows = tc ? kKvTcRows : max_rows <= 8 ? 8 : 16;
+  const int live_rows = (int)(max_rows < pl.rows ? max_rows : pl.rows);
   const int64_t cap = (int64_t)a->max_pages * a->page_size;
   int64_t len = a->max_len < cap ? a->max_len : cap;
   if (len < 1) len = 1;
-  const int64_t work = (int64_t)a->batch * a->n_kv_heads * gl_cdiv(max_rows, pl.rows) * gl_cdiv(len, kKvTile);
-  const int64_t most = (int64_t)gl_num_sms() * (tc ? 1 : pl.rows == 16 ? 3 : 2);
+  const int64_t units = (int64_t)a->batch * a->n_kv_heads * gl_cdiv(max_rows, pl.rows), work = units * gl_cdiv(len, kKvTile);
+  int64_t most = (int64_t)gl_num_sms() * (tc ? 1 : pl.rows == 8 ? 3 : 2);
+  if (most > kJoinMax) most = kJoinMax;
   pl.blocks = (int)(work < most ? work : most);
+  // units cut into many parts are joined by a block per row, others by one per 8 rows
+  const int y = pl.blocks > 16 * units ? live_rows : (live_rows + 7) / 8;
+  pl.join_y = y < 16 ? y : 16;
   return pl;
 }
 
@@ -603,7 +629,7 @@ int check_attend(const gl_kv_args* a) {
 
 uint64_t workspace_of(const gl_kv_args* a, const Plan& pl) {
   if (pl.blocks <= 1) return 0;
-  return 2ull * (uint64_t)pl.blocks * (uint64_t)pl.rows * (uint64_t)(a->head_dim * 4 + 8);
+  return (uint64_t)pl.blocks * (2ull * (uint64_t)pl.rows * (uint64_t)(a->head_dim * 4 + 8) + sizeof(KvCut));
 }
 
 }  // namespace
@@ -650,9 +676,10 @@ extern "C" int gl_kv_attend(const gl_kv_args* a, void* stream) {
   p.blocks = pl.blocks;
   p.page_shift = (a->page_size & (a->page_size - 1)) == 0 ? __builtin_ctz((unsigned)a->page_size) : -1;
   p.part_o = (float*)a->workspace;
+  p.cuts = need > 0 ? reinterpret_cast<KvCut*>((uint8_t*)a->workspace + 2ull * pl.blocks * pl.rows * (a->head_dim * 4 + 8)) : nullptr;
   p.part_ml = need > 0 ? reinterpret_cast<float2*>(p.part_o + 2ll * pl.blocks * pl.rows * a->head_dim) : nullptr;
   cudaStream_t st = (cudaStream_t)stream;
   if (a->head_dim == 128)
-    return a->x_dtype == GL_BF16 ? launch_all<128, __nv_bfloat16>(p, a, pl.rows, pl.live_rows, st) : launch_all<128, __half>(p, a, pl.rows, pl.live_rows, st);
-  return a->x_dtype == GL_BF16 ? launch_all<64, __nv_bfloat16>(p, a, pl.rows, pl.live_rows, st) : launch_all<64, __half>(p, a, pl.rows, pl.live_rows, st);
+    return a->x_dtype == GL_BF16 ? launch_all<128, __nv_bfloat16>(p, a, pl, st) : launch_all<128, __half>(p, a, pl, st);
+  return a->x_dtype == GL_BF16 ? launch_all<64, __nv_bfloat16>(p, a, pl, st) : launch_all<64, __half>(p, a, pl, st);
 }

@@ -2,6 +2,11 @@
 #pragma once
 #include "gl_kv.cuh"
 
+// what a block says about the units that its borders cut: bit 0: its last piece begins a unit and does not finish it (the unit:
+// first row of the sequence's tokens, head, first row, rows); bit 1: its first piece goes on with a unit; bit 2: and finishes it
+struct alignas(16) KvCut {
+  int32_t flags, first, head, row0, rows, pad[3];
+};
 struct KvAttendParams {
   KvBatch kb;
   const uint8_t *k_codes, *v_codes, *k_zeros, *v_zeros;
@@ -11,6 +16,7 @@ struct KvAttendParams {
   const uint8_t* mask;
   float* part_o;               // [2 * blocks][rows of a unit][D], unnormalised
   float2* part_ml;             // [2 * blocks][rows of a unit]: maximum and sum (0: nothing seen)
+  KvCut* cuts;                 // [blocks]
   int64_t q_sn, q_sh, mask_stride;
   int32_t mask_cols, hq, group, page_shift, blocks;
   float scale_log2;
@@ -37,7 +43,8 @@ __device__ __forceinline__ uint32_t kv_slot32(const KvBatch& kb, int page, int h
 // tokens.  All units' tiles stand in one line (sequence, kv head, row block, tile), and block i of n takes the i-th of n
 // equal pieces of the line: lengths may differ as they like, every block gets the same number of tiles, and a unit is cut
 // only where a block ends.  A block whose piece holds a whole unit writes the unit's result; the part of a unit that it starts in
-// the middle of goes to its scratch slot 2 i, the part that it does not finish to slot 2 i + 1, and kv_attend_join_kernel joins.
+// the middle of goes to its scratch slot 2 i, the part that it does not finish to slot 2 i + 1, and kv_attend_join_kernel joins
+// them by what the blocks say in `cuts`.
 // Nobody waits for anybody.  The lengths are on the device, so every block adds them up for itself.
 constexpr int kKvTile = 128;
 
@@ -67,11 +74,6 @@ struct KvShare {
   int more;
   __device__ __forceinline__ KvShare(int64_t t, int blocks) : total(t), each(kv_div(t, blocks)), more((int)(t - each * blocks)) {}
   __device__ __forceinline__ int64_t begin(int i) const { return each * i + min(i, more); }
-  // the block whose piece holds tile x < total
-  __device__ __forceinline__ int owner(int64_t x) const {
-    const int64_t y = x - more * (each + 1);
-    return (int)(y < 0 ? kv_div(x, each + 1) : more + kv_div(y, each));
-  }
 };
 // place in the line: sequence, and tiles of the sequence before it
 struct KvPlace {
@@ -134,6 +136,7 @@ struct KvPiece {
   int head, row0, rows;            // kv head; first row of the unit and its live rows
   int t0, t1;                      // tiles of this piece that some row may see (t1 <= t0: none)
   bool whole;                      // the unit's tiles are all in this piece
+  bool ends;                       // its last ones are
   int slot;                        // else: scratch slot of its part
 };
 // walks a block's piece of the line, unit by unit
@@ -148,6 +151,19 @@ template <int ROWS> struct KvWalk {
     const KvShare share(pl.total, p.blocks);
     left = b < 0 ? 0 : share.begin(i + 1) - share.begin(i);
     left_valid = 0;
+  }
+  // adds a piece to what the block says about its borders
+  static __device__ __forceinline__ void note(KvCut& cut, const KvPiece& pc) {
+    if (pc.whole) return;
+    if ((pc.slot & 1) == 0) {
+      cut.flags |= pc.ends ? 6 : 2;
+    } else {
+      cut.flags |= 1;
+      cut.first = pc.s.first;
+      cut.head = pc.head;
+      cut.row0 = pc.row0;
+      cut.rows = pc.rows;
+    }
   }
   __device__ __forceinline__ bool next(const KvAttendParams& p, int i, KvPiece& pc) {
     if (left <= 0) return false;
@@ -170,7 +186,8 @@ template <int ROWS> struct KvWalk {
     pc.head = head;
     pc.row0 = rb * ROWS;
     pc.rows = min(ROWS, s.new_b * p.group - pc.row0);
-    pc.whole = t0 == 0 && t1 == s.tiles;
+    pc.ends = t1 == s.tiles;
+    pc.whole = t0 == 0 && pc.ends;
     pc.slot = 2 * i + (t0 == 0 ? 1 : 0);
     // without a mask nothing behind the last row's own token is seen
     const int t_hi = (pc.row0 + pc.rows - 1) / p.group;
@@ -219,6 +236,10 @@ template <typename T> __device__ __forceinline__ uint32_t kv_pair(float a, float
 template <typename T, int N> __device__ __forceinline__ void kv_store_n(T* dst, const float (&v)[N]) {
   if constexpr (N == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(kv_pair<T>(v[0], v[1]), kv_pair<T>(v[2], v[3]));
   else *reinterpret_cast<uint32_t*>(dst) = kv_pair<T>(v[0], v[1]);
+}
+template <int N> __device__ __forceinline__ void kv_load_n(const float* src, float (&v)[N]) {
+  if constexpr (N == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+  else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
 }
 // a / l, rounded once to 16 bits; a row that saw nothing (l = 0) gives zeros
 template <typename T> __device__ __forceinline__ void kv_store4(T* dst, float4 a, float l) {

@@ -322,7 +322,7 @@ __device__ __forceinline__ void mma_role(const KvAttendParams& p, Shared& sh, ui
   const uint32_t q_lo = (uint32_t)qd, k_lo = (uint32_t)kd, k_hi = (uint32_t)(kd >> 32), v_lo = (uint32_t)vd, v_hi = (uint32_t)(vd >> 32);
   KvPiece pc;
   int n0 = 0;                                  // tiles of earlier pieces
-  uint32_t q_phase = 0, p_phase[2] = {0, 0};
+  uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
   while (walk.next(p, blockIdx.x, pc)) {
     const int n = pc.t1 - pc.t0;
     if (n <= 0) continue;
@@ -342,9 +342,10 @@ __device__ __forceinline__ void mma_role(const KvAttendParams& p, Shared& sh, ui
       if (!both || s == 1) tc_commit(&sh.k_empty[st]);
       return true;
     };
-    for (int s = 0; s < 2; ++s)
-      if (!mbar_wait_spin(&sh.q_full[s], q_phase, abort, nullptr, 0)) return;
-    q_phase ^= 1;
+    for (int s = 0; s < 2 && s < events; ++s) {                          // (a stream without a tile loads no queries)
+      if (!mbar_wait_spin(&sh.q_full[s], q_phase[s], abort, nullptr, 0)) return;
+      q_phase[s] ^= 1;
+    }
     tc_fence_after();
     for (int e = 0; e < 2 && e < events; ++e)
       if (!scores(e)) return;
@@ -379,7 +380,9 @@ __device__ __forceinline__ void stream_role(const KvAttendParams& p, Shared& sh,
   int n0 = 0, merges = 0;
   uint32_t s_phase = 0, o_phase = 0;
   bool ok = true;
+  KvCut cut{};
   while (walk.next(p, blockIdx.x, pc)) {
+    KvWalk<kKvTcRows>::note(cut, pc);
     const int n = pc.t1 - pc.t0 > 0 ? pc.t1 - pc.t0 : 0;
     const bool both = pc.rows > 128;
     const int r = both ? s * 128 + row : row;                    // row of the unit
@@ -387,7 +390,7 @@ __device__ __forceinline__ void stream_role(const KvAttendParams& p, Shared& sh,
     const int rr = pc.row0 + (live ? r : 0), tok = rr / p.group, head = pc.head * p.group + (rr - tok * p.group);
     float m_used = -INFINITY, l = 0.f;
     const int mine = both ? n : s == 0 ? (n + 1) / 2 : n / 2;
-    if (n > 0 && ok) {
+    if (mine > 0 && ok) {
       // ---- queries: fp16 by a power of two, into this stream's swizzled tile
       if (merges > 0) ok = warp_wait(&sh.x_empty, (merges - 1) & 1, abort);
       const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)(pc.s.first + tok) * p.q_sn + (int64_t)head * p.q_sh;
@@ -555,7 +558,7 @@ __device__ __forceinline__ void stream_role(const KvAttendParams& p, Shared& sh,
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.p_full[s]);
       }
-      if (mine > 0 && ok) {
+      if (ok) {
         ok = warp_wait(&sh.o_full[s], o_phase, abort);
         o_phase ^= 1;
         tc_fence_after();
@@ -650,6 +653,7 @@ __device__ __forceinline__ void stream_role(const KvAttendParams& p, Shared& sh,
     if (merge) ++merges;
     n0 += n;
   }
+  if (threadIdx.x == 0 && p.cuts != nullptr) p.cuts[blockIdx.x] = cut;
 }
 
 template <int D, int FMT, typename T>

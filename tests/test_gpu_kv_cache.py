@@ -173,7 +173,7 @@ def _check_attend(cache, table, ctx, new, q, mask, out, scale=None, rounds_codes
     rounds_codes: the kernel for many rows rounds scaled values and keys to fp16: 2^-11 of sum p |v| for the values, and for
     the keys twice (numerator, denominator) what score_slack64 says; its smallest weights have 2^-31 of the largest as their
     last normal order, 2^8 times the other kernel's floor."""
-    rounds_codes = rounds_codes or max(new) * (q.shape[1] // cache.n_kv_heads) > 32
+    rounds_codes = rounds_codes or max(new) * (q.shape[1] // cache.n_kv_heads) > 16
     at = 0
     for b, (c, t) in enumerate(zip(ctx, new)):
         if t == 0:
@@ -207,6 +207,9 @@ SHAPES = [  # hq, hkv, page, cached tokens, new tokens
     (16, 2, 32, [300, 0], [64, 33]),
     (5, 1, 128, [1000], [40]),
     (32, 2, 64, [0, 150], [100, 60]),
+    # several pieces per block: many sequences of one or two tiles; few long ones; units of one and of two row blocks mixed
+    (16, 4, 16, [17 * i % 150 for i in range(48)], [1 + i % 5 for i in range(48)]),
+    (24, 8, 32, [1400, 90, 2100, 700], [40, 1, 45, 100]),
 ]
 
 
