@@ -86,13 +86,17 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 3 : 2) kv_attend_mma_ke
     const int mine = (tiles - warp + kWarps - 1) / kWarps;              // tiles warp, warp + 4, ..
 
     // ---- tokens of a tile into shared memory, kStages - 1 tiles ahead
-    auto slot_of = [&](int i) -> uint32_t {                             // lane's token of the warp's i-th tile
+    int page_next = -1, place_next = 0;                                 // lane's token of the tile that is issued next: its
+    auto look_up = [&](int i) {                                         // page number is not touched before then
       const int pos = c0 + (warp + i * kWarps) * kTile + lane;
-      if (i >= mine || pos >= c1) return kNoSlot;
-      const int pi = p.page_shift >= 0 ? pos >> p.page_shift : pos / kb.page_size;
-      return kv_slot32(kb, kb.page_table[pt_row + pi], kvh, pos - pi * kb.page_size);
+      page_next = -1;
+      if (i < mine && pos < c1) {
+        const int pi = p.page_shift >= 0 ? pos >> p.page_shift : pos / kb.page_size;
+        place_next = pos - pi * kb.page_size;
+        page_next = __ldg(kb.page_table + pt_row + pi);
+      }
     };
-    uint32_t slot_next = slot_of(0);
+    look_up(0);
     uint32_t z_pend = 0;
     int z_stage = -1;
     auto put_zeros = [&]() {
@@ -107,9 +111,9 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 3 : 2) kv_attend_mma_ke
       if (i < mine) {
         const int st = i % kStages;
         const uint32_t at = ring_u + st * S::STAGE;
-        const uint32_t slot = slot_next, slot0 = __shfl_sync(0xffffffffu, slot, 0);
+        const uint32_t slot = kv_slot32(kb, page_next, kvh, place_next), slot0 = __shfl_sync(0xffffffffu, slot, 0);
         const bool live = slot != kNoSlot;
-        slot_next = slot_of(i + 1);
+        look_up(i + 1);
         if (__all_sync(0xffffffffu, slot == slot0 + lane && live)) {              // 32 rows in a row: a tile inside one page
           const uint8_t *ks = p.k_codes + (int64_t)slot0 * RB + lane * 16, *vs = p.v_codes + (int64_t)slot0 * RB + lane * 16;
 #pragma unroll
@@ -453,110 +457,133 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 3 : 2) kv_attend_mma_ke
 }
 
 // Joins the parts of the units that block borders cut: blocks (i, *) look after the unit that block i began and did not
-// finish.  Few parts: a warp per row, 8 rows at a time; many (one long sequence): a block per row, warp w takes parts w, w + 8, ..
+// finish.  Few parts: a warp per row; many (one long sequence): a block per row,
+// warp w takes parts w, w + WARPS, ..
 constexpr int kJoinMax = 1024;                 // thread blocks of a launch, at most
-template <int ROWS, int D, typename T>
-__global__ void __launch_bounds__(256) kv_attend_join_kernel(const KvAttendParams p) {
-  __shared__ float4 acc_s[8][D / 4];
-  __shared__ float2 red[8];
+template <int ROWS, int D, typename T, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) kv_attend_join_kernel(const KvAttendParams p) {
+  __shared__ float4 acc_s[WARPS][D / 4];
+  __shared__ float2 red[WARPS];
   __shared__ float weight[kJoinMax];
   __shared__ int last;
   constexpr int V = D / 32;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, i0 = blockIdx.x;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   gl_launch_dependents();
   gl_grid_dependency_wait();
-  const KvCut cut = p.cuts[i0];
-  if ((cut.flags & 1) == 0) return;
-  // the unit's last part: the first later block that finishes what it goes on with (blocks in between hold nothing else)
-  if (tid == 0) last = p.blocks - 1;
-  __syncthreads();
-  for (int i = i0 + 1 + tid; i < p.blocks; i += 256) {
-    if (i > *(volatile int*)&last) break;
-    if (p.cuts[i].flags & 4) { atomicMin(&last, i); break; }
-  }
-  __syncthreads();
-  const int i1 = last, n = i1 - i0 + 1;
-  auto part = [&](int k) { return (int64_t)(k == 0 ? 2 * i0 + 1 : 2 * (i0 + k)) * ROWS; };
-  auto dst_of = [&](int r) {
-    const int rr = cut.row0 + r, t = rr / p.group;
-    return reinterpret_cast<T*>(p.out) + ((int64_t)(cut.first + t) * p.hq + cut.head * p.group + (rr - t * p.group)) * D;
-  };
-  // weight of a part: 0 where it saw nothing; a sum of NaN with the maximum -inf stays one
-  auto weight_of = [&](float2 ml, float top) { return ml.y == 0.f ? 0.f : ml.x == -INFINITY ? ml.y : kv_exp2(ml.x - top); };
+  // WARPS = 8: block x looks after the unit that block x of the main kernel began.  WARPS = 32, for few units: block x looks for
+  // the x-th cut unit, and the x + gridDim.x-th, ..
+  for (int x = blockIdx.x;; x += gridDim.x) {
+    int i0 = x;
+    if (WARPS == 32) {
+      const bool starts = tid < p.blocks && (p.cuts[tid].flags & 1);
+      const uint32_t who = __ballot_sync(0xffffffffu, starts);
+      __syncthreads();
+      if (tid == 0) last = -1;
+      if (lane == 0) red[warp].x = __int_as_float(__popc(who));
+      __syncthreads();
+      int before = __popc(who & ((1u << lane) - 1u));
+      for (int w = 0; w < warp; ++w) before += __float_as_int(red[w].x);
+      if (starts && before == x) last = tid;
+      __syncthreads();
+      i0 = last;
+      __syncthreads();
+      if (i0 < 0) return;
+    } else if (x >= p.blocks - 1) {
+      return;
+    }
+    const KvCut cut = p.cuts[i0];
+    if ((cut.flags & 1) == 0) continue;
+    // the unit's last part: the first later block that finishes what it goes on with (blocks in between hold nothing else)
+    if (tid == 0) last = p.blocks - 1;
+    __syncthreads();
+    for (int i = i0 + 1 + tid; i < p.blocks; i += WARPS * 32) {
+      if (i > *(volatile int*)&last) break;
+      if (p.cuts[i].flags & 4) { atomicMin(&last, i); break; }
+    }
+    __syncthreads();
+    const int i1 = last, n = i1 - i0 + 1;
+    auto part = [&](int k) { return (int64_t)(k == 0 ? 2 * i0 + 1 : 2 * (i0 + k)) * ROWS; };
+    auto dst_of = [&](int r) {
+      const int rr = cut.row0 + r, t = rr / p.group;
+      return reinterpret_cast<T*>(p.out) + ((int64_t)(cut.first + t) * p.hq + cut.head * p.group + (rr - t * p.group)) * D;
+    };
+    // weight of a part: 0 where it saw nothing; a sum of NaN with the maximum -inf stays one
+    auto weight_of = [&](float2 ml, float top) { return ml.y == 0.f ? 0.f : ml.x == -INFINITY ? ml.y : kv_exp2(ml.x - top); };
 
-  if (n <= 16) {
-    for (int r = blockIdx.y * 8 + warp; r < cut.rows; r += gridDim.y * 8) {
-      const float2 ml = lane < n ? p.part_ml[part(lane) + r] : make_float2(-INFINITY, 0.f);
-      float top = ml.y != 0.f ? ml.x : -INFINITY;
+    if (n <= 16) {
+      for (int r = blockIdx.y * WARPS + warp; r < cut.rows; r += gridDim.y * WARPS) {
+        const float2 ml = lane < n ? p.part_ml[part(lane) + r] : make_float2(-INFINITY, 0.f);
+        float top = ml.y != 0.f ? ml.x : -INFINITY;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float f = weight_of(ml, top);
+        float l = f == 0.f ? 0.f : ml.y * f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        float acc[V] = {};
+#pragma unroll 4
+        for (int k = 0; k < n; ++k) {
+          float x[V];
+          kv_load_n<V>(p.part_o + (part(k) + r) * D + lane * V, x);
+          const float w = __shfl_sync(0xffffffffu, f, k);
+#pragma unroll
+          for (int j = 0; j < V; ++j) acc[j] += w == 0.f ? 0.f : x[j] * w;
+        }
+        const float q = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[j] = l == 0.f ? 0.f : acc[j] * q;
+        kv_store_n<T, V>(dst_of(r) + lane * V, acc);
+      }
+      continue;
+    }
+    for (int r = blockIdx.y; r < cut.rows; r += gridDim.y) {
+      float top = -INFINITY;
+      for (int k = tid; k < n; k += WARPS * 32) {
+        const float2 ml = p.part_ml[part(k) + r];
+        if (ml.y != 0.f) top = fmaxf(top, ml.x);
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float f = weight_of(ml, top);
-      float l = f == 0.f ? 0.f : ml.y * f;
+      if (lane == 0) red[warp].x = top;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, red[w].x);
+      float l = 0.f;
+      for (int k = tid; k < n; k += WARPS * 32) {
+        const float2 ml = p.part_ml[part(k) + r];
+        const float f = weight_of(ml, top);
+        weight[k] = f;
+        l += f == 0.f ? 0.f : ml.y * f;
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      if (lane == 0) red[warp].y = l;
+      __syncthreads();
       float acc[V] = {};
-#pragma unroll 4
-      for (int k = 0; k < n; ++k) {
+#pragma unroll 8
+      for (int k = warp; k < n; k += WARPS) {
         float x[V];
         kv_load_n<V>(p.part_o + (part(k) + r) * D + lane * V, x);
-        const float w = __shfl_sync(0xffffffffu, f, k);
+        const float w = weight[k];
 #pragma unroll
         for (int j = 0; j < V; ++j) acc[j] += w == 0.f ? 0.f : x[j] * w;
       }
-      const float q = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-      for (int j = 0; j < V; ++j) acc[j] = l == 0.f ? 0.f : acc[j] * q;
-      kv_store_n<T, V>(dst_of(r) + lane * V, acc);
-    }
-    return;
-  }
-  for (int r = blockIdx.y; r < cut.rows; r += gridDim.y) {
-    float top = -INFINITY;
-    for (int k = tid; k < n; k += 256) {
-      const float2 ml = p.part_ml[part(k) + r];
-      if (ml.y != 0.f) top = fmaxf(top, ml.x);
-    }
+      for (int j = 0; j < V; ++j) reinterpret_cast<float*>(acc_s[warp])[lane * V + j] = acc[j];
+      __syncthreads();
+      if (tid < D / 4) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        l = 0.f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) red[warp].x = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; ++w) top = fmaxf(top, red[w].x);
-    float l = 0.f;
-    for (int k = tid; k < n; k += 256) {
-      const float2 ml = p.part_ml[part(k) + r];
-      const float f = weight_of(ml, top);
-      weight[k] = f;
-      l += f == 0.f ? 0.f : ml.y * f;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if (lane == 0) red[warp].y = l;
-    __syncthreads();
-    float acc[V] = {};
-#pragma unroll 8
-    for (int k = warp; k < n; k += 8) {
-      float x[V];
-      kv_load_n<V>(p.part_o + (part(k) + r) * D + lane * V, x);
-      const float w = weight[k];
-#pragma unroll
-      for (int j = 0; j < V; ++j) acc[j] += w == 0.f ? 0.f : x[j] * w;
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j) reinterpret_cast<float*>(acc_s[warp])[lane * V + j] = acc[j];
-    __syncthreads();
-    if (tid < D / 4) {
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-      l = 0.f;
-#pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        const float4 x = acc_s[w][tid];
-        a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
-        l += red[w].y;
+        for (int w = 0; w < WARPS; ++w) {
+          const float4 x = acc_s[w][tid];
+          a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+          l += red[w].y;
+        }
+        kv_store4<T>(dst_of(r) + tid * 4, a, l);
       }
-      kv_store4<T>(dst_of(r) + tid * 4, a, l);
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
@@ -575,22 +602,26 @@ int launch_fmt(const KvAttendParams& p, int fmt, int rows, cudaStream_t st) {
     default: return rows == 8 ? launch_mma<D, GL_KV_INT4, 1, T>(p, st) : launch_mma<D, GL_KV_INT4, 2, T>(p, st);
   }
 }
-template <int ROWS, int D, typename T>
-int launch_join(const KvAttendParams& p, int grid_y, cudaStream_t st) {
-  GL_CUDA_CHECK(gl_launch_pdl(kv_attend_join_kernel<ROWS, D, T>, dim3((unsigned)(p.blocks - 1), (unsigned)grid_y), dim3(256), 0, st, p));
-  return GL_OK;
-}
-
 struct Plan {
   int rows, blocks, join_y;      // rows of a unit, thread blocks of the main kernel, blocks per cut unit of the join
+  bool join_many;                // units are cut into many parts
+  int units;                     // .. then: an upper bound of the cut units
 };
+
+template <int ROWS, int D, typename T>
+int launch_join(const KvAttendParams& p, const Plan& pl, cudaStream_t st) {
+  const dim3 grid((unsigned)(pl.join_many ? pl.units : p.blocks - 1), (unsigned)pl.join_y);
+  if (pl.join_many) GL_CUDA_CHECK(gl_launch_pdl(kv_attend_join_kernel<ROWS, D, T, 32>, grid, dim3(1024), 0, st, p));
+  else GL_CUDA_CHECK(gl_launch_pdl(kv_attend_join_kernel<ROWS, D, T, 8>, grid, dim3(256), 0, st, p));
+  return GL_OK;
+}
 
 template <int D, typename T>
 int launch_all(const KvAttendParams& p, const gl_kv_args* a, const Plan& pl, cudaStream_t st) {
   if (int rc = pl.rows == kKvTcRows ? gl_kv_attend_tc_launch(p, D, a->format, a->x_dtype, st) : launch_fmt<D, T>(p, a->format, pl.rows, st)) return rc;
   if (p.blocks == 1) return GL_OK;
-  if (pl.rows == kKvTcRows) return launch_join<kKvTcRows, D, T>(p, pl.join_y, st);
-  return pl.rows == 8 ? launch_join<8, D, T>(p, pl.join_y, st) : launch_join<16, D, T>(p, pl.join_y, st);
+  if (pl.rows == kKvTcRows) return launch_join<kKvTcRows, D, T>(p, pl, st);
+  return pl.rows == 8 ? launch_join<8, D, T>(p, pl, st) : launch_join<16, D, T>(p, pl, st);
 }
 
 // Few rows per kv head: the mma.sync kernel, which holds 8 or 16 rows in registers (three or two blocks per SM); more: the
@@ -600,7 +631,7 @@ Plan plan_of(const gl_kv_args* a) {
   const int group = a->n_q_heads / a->n_kv_heads;
   int64_t max_rows = (int64_t)(a->max_new < a->n_tokens ? a->max_new : a->n_tokens) * group;
   if (max_rows < 1) max_rows = 1;
-  const bool tc = a->kernel_override == 2 || (a->kernel_override == 0 && max_rows > 16);
+  const bool tc = a->kernel_override == 2 || (a->kernel_override == 0 && max_rows > 32);
   pl.rows = tc ? kKvTcRows : max_rows <= 8 ? 8 : 16;
   const int live_rows = (int)(max_rows < pl.rows ? max_rows : pl.rows);
   const int64_t cap = (int64_t)a->max_pages * a->page_size;
@@ -611,7 +642,9 @@ Plan plan_of(const gl_kv_args* a) {
   if (most > kJoinMax) most = kJoinMax;
   pl.blocks = (int)(work < most ? work : most);
   // units cut into many parts are joined by a block per row, others by one per 8 rows
-  const int y = pl.blocks > 16 * units ? live_rows : (live_rows + 7) / 8;
+  pl.join_many = pl.blocks > 16 * units;
+  pl.units = pl.join_many ? (int)units : 0;
+  const int y = pl.join_many ? live_rows : (live_rows + 7) / 8;
   pl.join_y = y < 16 ? y : 16;
   return pl;
 }

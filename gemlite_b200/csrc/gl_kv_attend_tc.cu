@@ -30,11 +30,11 @@ constexpr int kThreads = 20 * 32;             // 17 warps work; 20 fill the five
 constexpr int kMeta = 4;                       // tiles' scalars and masks: a tile's are read before the second tile after it is converted
 constexpr float kOff = 7.f, kRaise = 8.f;
 
-struct alignas(16) Meta {                      // per 32 tokens; read as 16-byte vectors
-  float ks[4], vs_log2[4], vs_inv[4];
-  uint32_t k_apart[4], v_apart[4];             // the scales are in the arrays, not in the codes
+struct alignas(16) Meta {                      // read as 16-byte vectors
+  float ks[4], vs_log2[4], vs_inv[4];          // per 32 tokens
+  uint32_t k_apart[4], v_apart[4];             // scales are not in the codes, but only
   uint32_t valid[4];
-  float col_ks[128], col_lv[128], col_rv[128];
+  float col_ks[128], col_lv[128], col_rv[128]; // per token, for tiles that are not treated as a whole
 };
 
 template <int D> struct Lay {
@@ -84,14 +84,15 @@ __device__ __forceinline__ uint32_t scaled(uint32_t x, uint32_t hi2, uint32_t lo
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// 32 lanes x 8 columns (x 4 for the store), complete on return: for the paths that are kept small rather than fast
-__device__ __forceinline__ void tmem_ld_8(uint32_t taddr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
+// 32 lanes x 16 columns (x 8 for the store): for the paths that are kept small
+__device__ __forceinline__ void tmem_ld_16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                 "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ void tmem_st_4(uint32_t taddr, const uint32_t (&r)[4]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};\n\ttcgen05.wait::st.sync.aligned;"
-               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+__device__ __forceinline__ void tmem_st_8(uint32_t taddr, const uint32_t (&r)[8]) {      // tmem_st_wait() must follow
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 __device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&r)[16]) {      // tmem_st_wait() must follow
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
@@ -289,15 +290,12 @@ __device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh
         m.valid[w] = valid;
       }
     }
-    if (apart || bad) {
-      const float v = apart ? (none ? 1e-30f : scale) : pow2(e);         // (folded already: the power of two is left)
-      const bool is_bad = (bad >> lane) & 1u;
-      if (values) {
-        m.col_lv[w * 32 + lane] = is_bad ? __int_as_float(0x7fc00000) : __log2f(v);
-        m.col_rv[w * 32 + lane] = __frcp_rn(v);
-      } else {
-        m.col_ks[w * 32 + lane] = scale;
-      }
+    if (values) {
+      const float v = none ? 1e-30f : scale;
+      m.col_lv[w * 32 + lane] = (bad >> lane) & 1u ? __int_as_float(0x7fc00000) : apart ? __log2f(v) : (float)e;
+      m.col_rv[w * 32 + lane] = apart ? __frcp_rn(v) : pow2(-e);
+    } else {
+      m.col_ks[w * 32 + lane] = apart ? scale : pow2(e);
     }
     fence_proxy_async_smem();
     __syncwarp();
@@ -388,6 +386,7 @@ __device__ __forceinline__ void stream_role(const KvAttendParams& p, Shared& sh,
     const int r = both ? s * 128 + row : row;                    // row of the unit
     const bool live = r < pc.rows;
     const int rr = pc.row0 + (live ? r : 0), tok = rr / p.group, head = pc.head * p.group + (rr - tok * p.group);
+    const bool any_live = __any_sync(0xffffffffu, live);
     float m_used = -INFINITY, l = 0.f;
     const int mine = both ? n : s == 0 ? (n + 1) / 2 : n / 2;
     if (mine > 0 && ok) {
@@ -438,6 +437,12 @@ __device__ __forceinline__ void stream_role(const KvAttendParams& p, Shared& sh,
         if (!ok) break;
         s_phase ^= 1;
         tc_fence_after();
+        if (!any_live) {                                              // 32 rows of nobody: their weights may be anything
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.p_full[s]);
+          continue;
+        }
         const int tile0 = (pc.t0 + j) * kKvTile;
         const uint4 vld = *reinterpret_cast<const uint4*>(meta.valid), ka = *reinterpret_cast<const uint4*>(meta.k_apart), va = *reinterpret_cast<const uint4*>(meta.v_apart);
         const bool full = (ka.x | ka.y | ka.z | ka.w | va.x | va.y | va.z | va.w) == 0 && (vld.x & vld.y & vld.z & vld.w) == 0xffffffffu &&
@@ -461,10 +466,9 @@ __device__ __forceinline__ void stream_role(const KvAttendParams& p, Shared& sh,
         }
         // ---- the tile's maximum.  (The paths for tiles that are not full are rolled up: unrolled, the kernel outgrew the
         // instruction cache and ran at less than half its speed.)
-        auto exponent = [&](float sc, int col) {
-          const int w = col >> 5;
-          return (meta.k_apart[w] ? sc * meta.col_ks[col] * qs : sc * (qs * meta.ks[w])) + (meta.v_apart[w] ? meta.col_lv[col] : meta.vs_log2[w]);
-        };
+        // columns c .. c + 15 that this row sees; whether any token of theirs exists
+        auto seen16 = [&](int c) { return ((c < 64 ? (c < 32 ? seen[0] : seen[1]) : (c < 96 ? seen[2] : seen[3])) >> (c & 31)) & 0xffffu; };
+        auto there16 = [&](int c) { return (meta.valid[c >> 5] >> (c & 31)) & 0xffffu; };
         float t_top = -INFINITY;
         if (full) {
           uint32_t x[32];
@@ -479,12 +483,19 @@ __device__ __forceinline__ void stream_role(const KvAttendParams& p, Shared& sh,
           }
         } else {
 #pragma unroll 1
-          for (int c = 0; c < 128; c += 8) {
-            uint32_t y[8];
-            tmem_ld_8(ts + c, y);
-            const uint32_t sw = (c < 64 ? (c < 32 ? seen[0] : seen[1]) : (c < 96 ? seen[2] : seen[3])) >> (c & 31);
+          for (int c = 0; c < 128; c += 16) {
+            if (there16(c) == 0) continue;
+            uint32_t y[16];
+            tmem_ld_16(ts + c, y);
+            const uint32_t sw = seen16(c);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) t_top = (sw >> k) & 1u ? fmaxf(t_top, exponent(__uint_as_float(y[k]), c + k)) : t_top;
+            for (int k = 0; k < 16; k += 4) {
+              const float4 ks = *reinterpret_cast<const float4*>(meta.col_ks + c + k), lv = *reinterpret_cast<const float4*>(meta.col_lv + c + k);
+              const float t0 = fmaf(__uint_as_float(y[k]) * ks.x, qs, lv.x), t1 = fmaf(__uint_as_float(y[k + 1]) * ks.y, qs, lv.y);
+              const float t2 = fmaf(__uint_as_float(y[k + 2]) * ks.z, qs, lv.z), t3 = fmaf(__uint_as_float(y[k + 3]) * ks.w, qs, lv.w);
+              t_top = fmaxf(t_top, fmaxf(fmaxf((sw >> k) & 1u ? t0 : -INFINITY, (sw >> (k + 1)) & 1u ? t1 : -INFINITY),
+                                         fmaxf((sw >> (k + 2)) & 1u ? t2 : -INFINITY, (sw >> (k + 3)) & 1u ? t3 : -INFINITY)));
+            }
           }
         }
         const bool raise = t_top > m_used + kRaise || (m_used == -INFINITY && t_top != -INFINITY);
@@ -534,24 +545,28 @@ __device__ __forceinline__ void stream_role(const KvAttendParams& p, Shared& sh,
           tmem_st_wait();
         } else {
 #pragma unroll 1
-          for (int c = 0; c < 128; c += 8) {
-            uint32_t y[8], pk[4];
-            tmem_ld_8(ts + c, y);
-            const uint32_t sw = (c < 64 ? (c < 32 ? seen[0] : seen[1]) : (c < 96 ? seen[2] : seen[3])) >> (c & 31);
-            const bool apart = meta.v_apart[c >> 5] != 0;
-            const float inv_vs = meta.vs_inv[c >> 5];
-            float e[8];
+          for (int c = 0; c < 128; c += 16) {
+            uint32_t pk[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (there16(c) != 0) {
+              uint32_t y[16];
+              tmem_ld_16(ts + c, y);
+              const uint32_t sw = seen16(c);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              e[k] = (sw >> k) & 1u ? kv_exp2(exponent(__uint_as_float(y[k]), c + k) + to_p) : 0.f;
-              l += (sw >> k) & 1u ? e[k] * (apart ? meta.col_rv[c + k] : inv_vs) : 0.f;
+              for (int k = 0; k < 16; k += 4) {
+                const float4 ks = *reinterpret_cast<const float4*>(meta.col_ks + c + k), lv = *reinterpret_cast<const float4*>(meta.col_lv + c + k),
+                             rv = *reinterpret_cast<const float4*>(meta.col_rv + c + k);
+                // (a token that is not seen has the weight 0, whatever its scale)
+                const float e0 = (sw >> k) & 1u ? kv_exp2(fmaf(__uint_as_float(y[k]) * ks.x, qs, lv.x) + to_p) : 0.f;
+                const float e1 = (sw >> (k + 1)) & 1u ? kv_exp2(fmaf(__uint_as_float(y[k + 1]) * ks.y, qs, lv.y) + to_p) : 0.f;
+                const float e2 = (sw >> (k + 2)) & 1u ? kv_exp2(fmaf(__uint_as_float(y[k + 2]) * ks.z, qs, lv.z) + to_p) : 0.f;
+                const float e3 = (sw >> (k + 3)) & 1u ? kv_exp2(fmaf(__uint_as_float(y[k + 3]) * ks.w, qs, lv.w) + to_p) : 0.f;
+                l += ((sw >> k) & 1u ? e0 * rv.x : 0.f) + ((sw >> (k + 1)) & 1u ? e1 * rv.y : 0.f) + ((sw >> (k + 2)) & 1u ? e2 * rv.z : 0.f) + ((sw >> (k + 3)) & 1u ? e3 * rv.w : 0.f);
+                pk[k >> 1] = kv_pair<__half>(e0, e1);
+                pk[(k >> 1) + 1] = kv_pair<__half>(e2, e3);
+              }
             }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const __half2 hh = __floats2half2_rn(e[2 * k], e[2 * k + 1]);
-              pk[k] = *reinterpret_cast<const uint32_t*>(&hh);
-            }
-            tmem_st_4(ts + c / 2, pk);
+            tmem_st_8(ts + c / 2, pk);                                // (columns whose scores have been read)
+            tmem_st_wait();
           }
         }
         tc_fence_before();

@@ -23,33 +23,39 @@ def norm64(x, w, eps):
     return x if w is None else x / torch.sqrt((x * x).mean(-1, keepdim=True) + eps) * w.double()
 
 
+def _rows_of(cache, page_table, b, count):
+    """(pages, places, there) of the first `count` tokens of sequence b."""
+    p = torch.arange(count, device=page_table.device)
+    col = p // cache.page_size
+    inside = col < page_table.shape[1]
+    page = page_table[b].long()[col.clamp(max=max(page_table.shape[1] - 1, 0))]
+    there = inside & (page >= 0) & (page < cache.num_pages)
+    return torch.where(there, page, 0), p % cache.page_size, there
+
+
 def held64(cache, which, page_table, b, count):
     """[count, heads, d] fp64: what the cache holds of the first `count` tokens of sequence b (missing pages: NaN)."""
-    codes, scales = getattr(cache, which + "_codes"), getattr(cache, which + "_scales")
-    ps, out = cache.page_size, []
-    for p in range(count):
-        page = int(page_table[b, p // ps]) if p // ps < page_table.shape[1] else -1
-        if not 0 <= page < cache.num_pages:
-            out.append(torch.full((cache.n_kv_heads, cache.head_dim), math.nan, dtype=torch.float64, device=codes.device))
-            continue
-        c, s = codes[page, :, p % ps], scales[page, :, p % ps].double()[:, None]
-        if cache.kv_format == "fp8":
-            x = c.view(torch.float8_e4m3fn).double()
-        elif cache.kv_format == "int8":
-            x = c.view(torch.int8).double()
-        else:
-            z = getattr(cache, which + "_zeros")[page, :, p % ps].double()[:, None]
-            x = torch.stack([c % 16, c // 16], -1).flatten(-2).double() - z
-        out.append(x * s)
-    return torch.stack(out) if out else torch.empty((0, cache.n_kv_heads, cache.head_dim), dtype=torch.float64, device=codes.device)
+    codes = getattr(cache, which + "_codes")
+    if count == 0:
+        return torch.empty((0, cache.n_kv_heads, cache.head_dim), dtype=torch.float64, device=codes.device)
+    page, place, there = _rows_of(cache, page_table, b, count)
+    c, s = codes[page, :, place], getattr(cache, which + "_scales")[page, :, place].double()[..., None]
+    if cache.kv_format == "fp8":
+        x = c.view(torch.float8_e4m3fn).double()
+    elif cache.kv_format == "int8":
+        x = c.view(torch.int8).double()
+    else:
+        x = torch.stack([c % 16, c // 16], -1).flatten(-2).double() - getattr(cache, which + "_zeros")[page, :, place].double()[..., None]
+    return torch.where(there[:, None, None], x * s, math.nan)
 
 
 def scales64(cache, which, page_table, b, count):
     """[count, heads] fp64: the scales of the first `count` tokens of sequence b (missing pages: NaN)."""
-    s, ps = getattr(cache, which + "_scales"), cache.page_size
-    rows = [s[int(page_table[b, p // ps]), :, p % ps] if 0 <= int(page_table[b, p // ps]) < cache.num_pages else torch.full_like(s[0, :, 0], math.nan)
-            for p in range(count)]
-    return torch.stack(rows).double() if rows else torch.empty((0, cache.n_kv_heads), dtype=torch.float64, device=s.device)
+    s = getattr(cache, which + "_scales")
+    if count == 0:
+        return torch.empty((0, cache.n_kv_heads), dtype=torch.float64, device=s.device)
+    page, place, there = _rows_of(cache, page_table, b, count)
+    return torch.where(there[:, None], s[page, :, place].double(), math.nan)
 
 
 def score_slack64(q, k, sees, scale):

@@ -173,14 +173,15 @@ def _check_attend(cache, table, ctx, new, q, mask, out, scale=None, rounds_codes
     rounds_codes: the kernel for many rows rounds scaled values and keys to fp16: 2^-11 of sum p |v| for the values, and for
     the keys twice (numerator, denominator) what score_slack64 says; its smallest weights have 2^-31 of the largest as their
     last normal order, 2^8 times the other kernel's floor."""
-    rounds_codes = rounds_codes or max(new) * (q.shape[1] // cache.n_kv_heads) > 16
+    rounds_codes = rounds_codes or max(new) * (q.shape[1] // cache.n_kv_heads) > 32
     at = 0
     for b, (c, t) in enumerate(zip(ctx, new)):
         if t == 0:
             continue
         cap = min(c + t, table.shape[1] * cache.page_size)
         k, v = held64(cache, "k", table, b, cap), held64(cache, "v", table, b, cap)
-        hole = torch.tensor([not 0 <= int(table[b, p // cache.page_size]) < cache.num_pages for p in range(cap)], device=DEV)
+        col = table[b, torch.arange(cap, device=DEV) // cache.page_size]
+        hole = (col < 0) | (col >= cache.num_pages)
         sees = torch.zeros((t, cap), dtype=torch.bool, device=DEV)
         sees[:, :min(c, cap)] = True
         own = torch.ones((t, t), device=DEV).tril().bool() if mask is None else torch.nn.functional.pad(mask[at:at + t].bool(), (0, t))[:, :t]
