@@ -52,184 +52,243 @@ struct WriteParams {
   uint8_t *codes[2], *zeros[2];
   float* scales[2];
   int64_t q_sn, q_sh, k_sn, k_sh, v_sn, v_sh;
-  int32_t hq, rot, interleaved, table_rows, norm_dtype;
+  int32_t hq, rot, table_rows, norm_dtype;
   float eps;
 };
 
 // One block per token (and slice of its heads): the token's rotation, its norm weights and its slot are fetched once and
-// serve all of its heads.  LPR lanes per row.  The order of the fp32 operations is the one of the formulas, without fused
-// multiply-adds, and the sum of squares is kept in fp64: a code next to a rounding border then does not depend on how
-// the row was spread over lanes.
-// 8192 tokens of 64 + 2 x 8 heads of 128 (323 MB): see the table in the file's last comment.
-template <typename T, int LPR, int FMT>
-__global__ void __launch_bounds__(256) kv_write_kernel(const WriteParams p) {
-  constexpr int D = LPR * 8, GROUPS = 256 / LPR;
-  const int n = blockIdx.x;
+// serve all of its heads.  LPR lanes per row of 8 channels each, taken as two pieces of 4 so that a channel and its partner in the
+// rotation are in the same lane.  Queries go four rows at a time: their sums of squares are reduced together, each lane then
+// takes the square root and the reciprocal of one row.
+//
+// The order of the fp32 operations is the one of the formulas, without fused multiply-adds, and the sum of squares is kept in
+// fp64: a code next to a rounding border then does not depend on how the row was spread over lanes.
+template <typename T, int LPR> struct Rows {
+  static constexpr int D = LPR * 8;
+  struct Raw { uint2 p, q; };
+  int a, b;                                    // first channel of each piece
+  __device__ __forceinline__ Raw load(const T* row) const { return Raw{*reinterpret_cast<const uint2*>(row + a), *reinterpret_cast<const uint2*>(row + b)}; }
+  static __device__ __forceinline__ void unpack(const Raw& r, float (&x)[8]) {
+    const uint32_t w[4] = {r.p.x, r.p.y, r.q.x, r.q.y};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = Half2Of<T>::up(w[j]);
+      x[2 * j] = f.x;
+      x[2 * j + 1] = f.y;
+    }
+  }
+};
+
+// a lane's 8 weights: two pieces of 4
+__device__ __forceinline__ void load_weights(const void* w, int dtype, int a, int b, float (&v)[8]) {
+  if (dtype == GL_FP32) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = reinterpret_cast<const float*>(w)[a + j];
+      v[4 + j] = reinterpret_cast<const float*>(w)[b + j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t x = reinterpret_cast<const uint16_t*>(w)[a + j], y = reinterpret_cast<const uint16_t*>(w)[b + j];
+      v[j] = dtype == GL_BF16 ? __uint_as_float(x << 16) : __half2float(__ushort_as_half((unsigned short)x));
+      v[4 + j] = dtype == GL_BF16 ? __uint_as_float(y << 16) : __half2float(__ushort_as_half((unsigned short)y));
+    }
+  }
+}
+
+// x / sqrt(mean x^2 + eps) * w of R rows (1 or 4) of a group of LPR lanes
+template <int R, int LPR>
+__device__ __forceinline__ void normalise(float (&x)[R][8], const float (&w)[8], float eps, unsigned gmask) {
+  const int lane = threadIdx.x % LPR;
+  double ss[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    ss[r] = 0.0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss[r] += (double)x[r][j] * (double)x[r][j];
+  }
+  double mine = ss[0];
+  int o = LPR / 2;
+  if constexpr (R == 4) {                      // halves of the group keep two rows each, quarters one
+    const bool up = lane & (LPR / 2), up2 = lane & (LPR / 4);
+    const double k0 = (up ? ss[2] : ss[0]) + __shfl_xor_sync(gmask, up ? ss[0] : ss[2], LPR / 2);
+    const double k1 = (up ? ss[3] : ss[1]) + __shfl_xor_sync(gmask, up ? ss[1] : ss[3], LPR / 2);
+    mine = (up2 ? k1 : k0) + __shfl_xor_sync(gmask, up2 ? k0 : k1, LPR / 4);
+    o = LPR / 8;
+  }
+  for (; o > 0; o >>= 1) mine += __shfl_xor_sync(gmask, mine, o);
+  const float mean = (float)(mine * (1.0 / (LPR * 8)));
+  const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(mean, eps)));
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float f = R == 1 ? inv : __shfl_sync(gmask, inv, ((threadIdx.x & 31) / LPR) * LPR + (r >> 1) * (LPR / 2) + (r & 1) * (LPR / 4));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[r][j] = __fmul_rn(__fmul_rn(x[r][j], f), w[j]);
+  }
+}
+template <bool INTER> __device__ __forceinline__ void rotate(float (&x)[8], const float (&cs)[4], const float (&sn)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float a = INTER ? x[2 * j] : x[j], b = INTER ? x[2 * j + 1] : x[4 + j];
+    x[INTER ? 2 * j : j] = __fsub_rn(__fmul_rn(a, cs[j]), __fmul_rn(b, sn[j]));
+    x[INTER ? 2 * j + 1 : 4 + j] = __fadd_rn(__fmul_rn(b, cs[j]), __fmul_rn(a, sn[j]));
+  }
+}
+
+template <typename T, int LPR, int FMT, bool INTER>
+__global__ void __launch_bounds__(256, 3) kv_write_kernel(const WriteParams p) {
+  constexpr int D = LPR * 8, GROUPS = 256 / LPR, R = 4;
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
   const unsigned gmask = (LPR == 16 ? 0xffffu : 0xffu) << ((threadIdx.x & 31) / LPR * LPR);
   gl_launch_dependents();
   gl_grid_dependency_wait();
-
-  // sequence of row n: how many sequences end at or before it
-  int b = 0, i = 0;
-  if (p.kb.q_offsets != nullptr) {
-    for (int base = 0; base < p.kb.batch; base += 256) {
-      const int t = base + threadIdx.x;
-      b += __syncthreads_count(t < p.kb.batch && p.kb.q_offsets[t + 1] <= n);
-    }
-    if (b >= p.kb.batch || n < p.kb.q_offsets[0]) return;
-    i = n - p.kb.q_offsets[b];
-  } else {
-    const int t = p.kb.n_tokens / p.kb.batch;
-    b = n / t;
-    i = n - b * t;
-  }
-  const int64_t pos_in_seq = (int64_t)max(p.kb.lens[b], 0) + i;
-  const int64_t slot0 = kv_slot(p.kb, b, 0, pos_in_seq);
-
-  // this lane's share of the rotation: cosine and sine of its 8 channels (interleaved: 4 pairs)
-  float cs[8], sn[8];
-  bool bad_pos = false;
+  // this lane's channels, and their norm weights
   const bool turns = lane * 8 < p.rot;
-  if (p.rot > 0) {
-    const int row = p.positions[n];
-    bad_pos = (unsigned)row >= (unsigned)p.table_rows;
-    if (turns && !bad_pos) {
-      const float* t = p.cos_sin + (int64_t)row * p.rot;
-      const int half = p.rot / 2;
-      const int at = p.interleaved ? lane * 4 : (lane * 8 < half ? lane * 8 : lane * 8 - half);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int e = p.interleaved ? at + j / 2 : at + j;
-        cs[j] = t[e];
-        sn[j] = t[half + e];
-      }
-    } else if (turns) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) { cs[j] = __int_as_float(0x7fc00000); sn[j] = cs[j]; }
-    }
-  }
-  const int partner = lane * 8 < p.rot / 2 ? p.rot / 16 : -(p.rot / 16);   // in lanes
+  Rows<T, LPR> rows;
+  rows.a = INTER || !turns ? lane * 8 : lane * 4;
+  rows.b = INTER || !turns ? lane * 8 + 4 : p.rot / 2 + lane * 4;
+  const int hq = p.q != nullptr ? p.hq : 0;
+  float wq[8], wk[8];
+  if (p.q_norm != nullptr) load_weights(p.q_norm, p.norm_dtype, rows.a, rows.b, wq);
+  if (p.k_norm != nullptr) load_weights(p.k_norm, p.norm_dtype, rows.a, rows.b, wk);
 
-  const int hq = p.q != nullptr ? p.hq : 0, rows = hq + 2 * p.kb.hkv;
-  float w[8];
-  int w_of = -1;
-  for (int r0 = blockIdx.y * GROUPS; r0 < rows; r0 += gridDim.y * GROUPS) {
-    const int r = r0 + group;
-    if (r >= rows) break;                     // whole groups leave together; the shuffles below name the group's lanes
-    const int kind = r < hq ? 0 : r < hq + p.kb.hkv ? 1 : 2, h = kind == 0 ? r : kind == 1 ? r - hq : r - hq - p.kb.hkv;
-    const T* src = kind == 0 ? reinterpret_cast<const T*>(p.q) + n * p.q_sn + h * p.q_sh
-                 : kind == 1 ? reinterpret_cast<const T*>(p.k) + n * p.k_sn + h * p.k_sh
-                             : reinterpret_cast<const T*>(p.v) + n * p.v_sn + h * p.v_sh;
-    const uint4 u = *reinterpret_cast<const uint4*>(src + lane * 8);
-    float x[8];
-    {
-      const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
+  for (int n = blockIdx.x; n < p.kb.n_tokens; n += gridDim.x) {
+    // what does not depend on the sequence first: the first rows, and the position
+    const T* q_src = reinterpret_cast<const T*>(p.q) + n * p.q_sn;
+    typename Rows<T, LPR>::Raw raw[R], raw_kv;
+    const int hkv = p.kb.hkv, kv_first = (int)(gridDim.y - 1 - blockIdx.y) * GROUPS + group;      // (slices take keys and values from the other end)
+    auto fetch_q = [&](int h0) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = Half2Of<T>::up(uw[j]);
-        x[2 * j] = f.x;
-        x[2 * j + 1] = f.y;
+      for (int r = 0; r < R; ++r) {
+        const int h = h0 + group + r * gridDim.y * GROUPS;
+        raw[r].p = raw[r].q = make_uint2(0, 0);
+        if (h < hq) raw[r] = rows.load(q_src + h * p.q_sh);
+      }
+    };
+    auto fetch_kv = [&](int r0) {
+      if (r0 < 2 * hkv) raw_kv = rows.load(r0 < hkv ? reinterpret_cast<const T*>(p.k) + n * p.k_sn + r0 * p.k_sh : reinterpret_cast<const T*>(p.v) + n * p.v_sn + (r0 - hkv) * p.v_sh);
+    };
+    fetch_q(blockIdx.y * GROUPS);
+    fetch_kv(kv_first);
+    const int at = p.rot > 0 ? p.positions[n] : 0;
+
+    // sequence of row n: how many sequences end at or before it
+    int b = 0, i = 0;
+    if (p.kb.q_offsets != nullptr) {
+      for (int base = 0; base < p.kb.batch; base += 32) {
+        const int t = base + (threadIdx.x & 31);
+        const unsigned done = __ballot_sync(0xffffffffu, t < p.kb.batch && p.kb.q_offsets[t + 1] <= n);
+        b += __popc(done);
+        if (done != 0xffffffffu) break;                      // ascending
+      }
+      if (b >= p.kb.batch || n < p.kb.q_offsets[0]) continue;
+      i = n - p.kb.q_offsets[b];
+    } else {
+      const int t = p.kb.n_tokens / p.kb.batch;
+      b = n / t;
+      i = n - b * t;
+    }
+    const int64_t slot0 = kv_slot(p.kb, b, 0, (int64_t)max(p.kb.lens[b], 0) + i);
+
+    // this lane's share of the rotation: the cosine and sine of four pairs
+    float cs[4], sn[4];
+    bool bad_pos = false;
+    if (p.rot > 0) {
+      bad_pos = (unsigned)at >= (unsigned)p.table_rows;
+      if (turns) {
+        const float* t = p.cos_sin + (bad_pos ? 0 : (int64_t)at * p.rot) + lane * 4;
+        const float4 c4 = *reinterpret_cast<const float4*>(t), s4 = *reinterpret_cast<const float4*>(t + p.rot / 2);
+        cs[0] = c4.x; cs[1] = c4.y; cs[2] = c4.z; cs[3] = c4.w;
+        sn[0] = s4.x; sn[1] = s4.y; sn[2] = s4.z; sn[3] = s4.w;
       }
     }
-    if (kind < 2) {
-      const void* nw = kind == 0 ? p.q_norm : p.k_norm;
-      if (nw != nullptr) {
-        if (w_of != kind) {
+    // ---- queries
+    if (hq > 0) {
+      T* dst = reinterpret_cast<T*>(p.q_out) + (int64_t)n * hq * D;
+      for (int h0 = blockIdx.y * GROUPS; h0 < hq; h0 += gridDim.y * GROUPS * R) {
+        float x[R][8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) w[j] = gl_load_as_float(nw, lane * 8 + j, p.norm_dtype);
-          w_of = kind;
-        }
-        double ss = 0.0;
+        for (int r = 0; r < R; ++r) rows.unpack(raw[r], x[r]);
+        if (h0 + gridDim.y * GROUPS * R < hq) fetch_q(h0 + gridDim.y * GROUPS * R);
+        if (p.q_norm != nullptr) normalise<R, LPR>(x, wq, p.eps, gmask);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss += (double)x[j] * (double)x[j];
+        for (int r = 0; r < R; ++r) {
+          const int h = h0 + group + r * gridDim.y * GROUPS;
+          if (turns) rotate<INTER>(x[r], cs, sn);
+          if (bad_pos)
 #pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(gmask, ss, o);
-        const float mean = (float)(ss * (1.0 / D));
-        const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(mean, p.eps)));
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(__fmul_rn(x[j], inv), w[j]);
-      }
-      if (p.rot > 0) {
-        if (p.interleaved) {
-          if (turns) {
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-              const float a = x[j], c = x[j + 1];
-              x[j] = __fsub_rn(__fmul_rn(a, cs[j]), __fmul_rn(c, sn[j]));
-              x[j + 1] = __fadd_rn(__fmul_rn(c, cs[j]), __fmul_rn(a, sn[j]));
-            }
-          }
-        } else {
-          const int from = (threadIdx.x & 31) + (turns ? partner : 0);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float other = __shfl_sync(gmask, x[j], from);
-            if (turns) {
-              const float own = __fmul_rn(x[j], cs[j]), turn = __fmul_rn(other, sn[j]);
-              x[j] = partner > 0 ? __fsub_rn(own, turn) : __fadd_rn(own, turn);
-            }
+            for (int j = 0; j < 8; ++j) x[r][j] = __int_as_float(0x7fc00000);
+          if (h < hq) {
+            *reinterpret_cast<uint2*>(dst + h * D + rows.a) = make_uint2(Half2Of<T>::down(x[r][0], x[r][1]), Half2Of<T>::down(x[r][2], x[r][3]));
+            *reinterpret_cast<uint2*>(dst + h * D + rows.b) = make_uint2(Half2Of<T>::down(x[r][4], x[r][5]), Half2Of<T>::down(x[r][6], x[r][7]));
           }
         }
-        if (bad_pos) {                        // channels that do not turn as well: no half-valid rows
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = __int_as_float(0x7fc00000);
-        }
       }
-    }
-    if (kind == 0) {
-      uint4 o;
-      o.x = Half2Of<T>::down(x[0], x[1]);
-      o.y = Half2Of<T>::down(x[2], x[3]);
-      o.z = Half2Of<T>::down(x[4], x[5]);
-      o.w = Half2Of<T>::down(x[6], x[7]);
-      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.q_out) + ((int64_t)n * p.hq + h) * D + lane * 8) = o;
-      continue;
     }
     if (slot0 < 0) continue;
-    const int which = kind - 1;
-    const int64_t slot = slot0 + (int64_t)h * p.kb.page_size;
-    // |x| as integers: infinities and NaN are the largest
-    uint32_t top = 0;
+
+    // ---- keys and values
+    for (int r0 = kv_first; r0 < 2 * hkv; r0 += gridDim.y * GROUPS) {
+      const int which = r0 < hkv ? 0 : 1, h = which ? r0 - hkv : r0;
+      float x[1][8];
+      rows.unpack(raw_kv, x[0]);
+      fetch_kv(r0 + gridDim.y * GROUPS);
+      if (which == 0) {
+        if (p.k_norm != nullptr) normalise<1, LPR>(x, wk, p.eps, gmask);
+        if (turns) rotate<INTER>(x[0], cs, sn);
+        if (bad_pos)                               // channels that do not turn as well: no half-valid rows
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(gmask, top, o));
-    const bool finite = top < 0x7f800000u;
-    if (FMT == GL_KV_INT4) {
-      float lo = 0.f, hi = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) { lo = fminf(lo, x[j]); hi = fmaxf(hi, x[j]); }
-#pragma unroll
-      for (int o = LPR / 2; o > 0; o >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(gmask, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(gmask, hi, o));
+          for (int j = 0; j < 8; ++j) x[0][j] = __int_as_float(0x7fc00000);
       }
-      const float scale = fmaxf(__fdiv_rn(__fsub_rn(hi, lo), 15.f), 1e-6f);
-      const float zero = fminf(fmaxf(rintf(__fdiv_rn(-lo, scale)), 0.f), 15.f);
-      uint32_t o = 0;
+      const int64_t slot = slot0 + (int64_t)h * p.kb.page_size;
+      // |x| as integers: infinities and NaN are the largest
+      uint32_t top = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float c = fminf(fmaxf(rintf(__fdiv_rn(x[j], scale)) + zero, 0.f), 15.f);
-        o |= (uint32_t)(int)c << (4 * j);
-      }
-      reinterpret_cast<uint32_t*>(p.codes[which] + slot * (D / 2))[lane] = finite ? o : 0u;
-      if (lane == 0) {
-        p.scales[which][slot] = finite ? scale : __int_as_float(0x7fc00000);
-        p.zeros[which][slot] = finite ? (uint8_t)(int)zero : (uint8_t)0;
-      }
-    } else {
-      const float qmax = FMT == GL_KV_FP8 ? 448.f : 127.f;
-      const float scale = fmaxf(__fdiv_rn(__uint_as_float(top), qmax), 1e-6f);
-      uint32_t o[2] = {0u, 0u};
+      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[0][j]) & 0x7fffffffu);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float c = fminf(fmaxf(__fdiv_rn(x[j], scale), -qmax), qmax);
-        const uint32_t byte = FMT == GL_KV_FP8 ? (uint32_t)__nv_cvt_float_to_fp8(c, __NV_SATFINITE, __NV_E4M3) : (uint32_t)(uint8_t)(int8_t)(int)rintf(c);
-        o[j >> 2] |= byte << (8 * (j & 3));
+      for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(gmask, top, o));
+      const bool finite = top < 0x7f800000u;
+      if (FMT == GL_KV_INT4) {
+        float lo = 0.f, hi = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { lo = fminf(lo, x[0][j]); hi = fmaxf(hi, x[0][j]); }
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) {
+          lo = fminf(lo, __shfl_xor_sync(gmask, lo, o));
+          hi = fmaxf(hi, __shfl_xor_sync(gmask, hi, o));
+        }
+        const float scale = fmaxf(__fdiv_rn(__fsub_rn(hi, lo), 15.f), 1e-6f);
+        const float zero = fminf(fmaxf(rintf(__fdiv_rn(-lo, scale)), 0.f), 15.f);
+        uint32_t o = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float c = fminf(fmaxf(rintf(__fdiv_rn(x[0][j], scale)) + zero, 0.f), 15.f);
+          o |= (uint32_t)(int)c << (4 * j);
+        }
+        if (!finite) o = 0u;
+        uint8_t* dst = p.codes[which] + slot * (D / 2);
+        *reinterpret_cast<uint16_t*>(dst + rows.a / 2) = (uint16_t)o;
+        *reinterpret_cast<uint16_t*>(dst + rows.b / 2) = (uint16_t)(o >> 16);
+        if (lane == 0) {
+          p.scales[which][slot] = finite ? scale : __int_as_float(0x7fc00000);
+          p.zeros[which][slot] = finite ? (uint8_t)(int)zero : (uint8_t)0;
+        }
+      } else {
+        const float qmax = FMT == GL_KV_FP8 ? 448.f : 127.f;
+        const float scale = fmaxf(__fdiv_rn(__uint_as_float(top), qmax), 1e-6f);
+        uint32_t o[2] = {0u, 0u};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float c = fminf(fmaxf(__fdiv_rn(x[0][j], scale), -qmax), qmax);
+          const uint32_t byte = FMT == GL_KV_FP8 ? (uint32_t)__nv_cvt_float_to_fp8(c, __NV_SATFINITE, __NV_E4M3) : (uint32_t)(uint8_t)(int8_t)(int)rintf(c);
+          o[j >> 2] |= byte << (8 * (j & 3));
+        }
+        uint8_t* dst = p.codes[which] + slot * D;
+        *reinterpret_cast<uint32_t*>(dst + rows.a) = finite ? o[0] : 0u;
+        *reinterpret_cast<uint32_t*>(dst + rows.b) = finite ? o[1] : 0u;
+        if (lane == 0) p.scales[which][slot] = finite ? scale : __int_as_float(0x7fc00000);
       }
-      reinterpret_cast<uint2*>(p.codes[which] + slot * D)[lane] = finite ? make_uint2(o[0], o[1]) : make_uint2(0u, 0u);
-      if (lane == 0) p.scales[which][slot] = finite ? scale : __int_as_float(0x7fc00000);
     }
   }
 }
@@ -239,68 +298,95 @@ struct ReadParams {
   const uint8_t *codes[2], *zeros[2];
   const float* scales[2];
   void* out[2];
-  int32_t max_len, out_dtype;
+  int32_t max_len, heads_shift;
 };
 
-// One lane per 16 channels of a row, keys and values of the same slot by the same lane.
+// One lane per 16 channels of a row, keys and values of the same slot by the same lane.  A block takes whole tokens (all heads of
+// one follow each other in the output) and several rows per lane, whose loads are issued together.
 template <int D, int FMT, typename O>
 __global__ void __launch_bounds__(256) kv_read_kernel(const ReadParams p) {
-  constexpr int LPR = D / 16, ROWS = 256 / LPR;
-  const int lane = threadIdx.x % LPR;
-  const int64_t t = (int64_t)blockIdx.x * ROWS + threadIdx.x / LPR;
-  const int h = blockIdx.y;
+  constexpr int LPR = D / 16, ROWS = 256 / LPR, N = 2;
+  const int lane = threadIdx.x % LPR, hkv = p.kb.hkv;
+  const int64_t row0 = (int64_t)blockIdx.x * (ROWS * N) + threadIdx.x / LPR;
   gl_launch_dependents();
   gl_grid_dependency_wait();
-  if (t >= p.max_len) return;
-  for (int b = blockIdx.z; b < p.kb.batch; b += gridDim.z) {
-    const int64_t slot = t < p.kb.lens[b] ? kv_slot(p.kb, b, h, t) : -1;
+  for (int b = blockIdx.y; b < p.kb.batch; b += gridDim.y) {
+    const int len = p.kb.lens[b];
+    int64_t slot[N], at[N];
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      float x[16];
-      if (slot >= 0) {
-        const float scale = p.scales[w][slot];
-        if (FMT == GL_KV_INT4) {
-          const uint2 u = *reinterpret_cast<const uint2*>(p.codes[w] + slot * (D / 2) + lane * 8);
-          const int zero = p.zeros[w][slot];
-          const uint32_t uw[2] = {u.x, u.y};
+    for (int i = 0; i < N; ++i) {
+      const int64_t row = row0 + i * ROWS;
+      const uint32_t t = p.heads_shift >= 0 ? (uint32_t)(row >> p.heads_shift) : (uint32_t)((uint64_t)row / (uint32_t)hkv);
+      const int h = (int)(row - (int64_t)t * hkv);
+      at[i] = t < (uint32_t)p.max_len ? row : -1;
+      slot[i] = at[i] >= 0 && (int64_t)t < len ? kv_slot(p.kb, b, h, t) : -1;
+    }
+    uint4 u[2][N];
+    float scale[2][N];
+    int zero[2][N];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) x[j] = (float)((int)((uw[j >> 3] >> (4 * (j & 7))) & 15u) - zero) * scale;
-        } else {
-          const uint4 u = *reinterpret_cast<const uint4*>(p.codes[w] + slot * D + lane * 16);
-          const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
+    for (int i = 0; i < N; ++i)
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const uint32_t byte = (uw[j >> 2] >> (8 * (j & 3))) & 255u;
-            x[j] = (FMT == GL_KV_FP8 ? gl_e4m3_to_float(byte) : (float)(int8_t)byte) * scale;
+      for (int w = 0; w < 2; ++w) {
+        u[w][i] = make_uint4(0, 0, 0, 0);
+        scale[w][i] = 0.f;
+        zero[w][i] = 0;
+        if (slot[i] >= 0) {
+          scale[w][i] = p.scales[w][slot[i]];
+          if (FMT == GL_KV_INT4) {
+            const uint2 x = *reinterpret_cast<const uint2*>(p.codes[w] + slot[i] * (D / 2) + lane * 8);
+            u[w][i].x = x.x;
+            u[w][i].y = x.y;
+            zero[w][i] = p.zeros[w][slot[i]];
+          } else {
+            u[w][i] = *reinterpret_cast<const uint4*>(p.codes[w] + slot[i] * D + lane * 16);
           }
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = 0.f;
       }
-      O* dst = reinterpret_cast<O*>(p.out[w]) + (((int64_t)b * p.max_len + t) * p.kb.hkv + h) * D + lane * 16;
-      if constexpr (sizeof(O) == 4) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) reinterpret_cast<float4*>(dst)[j] = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
-      } else {
-        uint32_t o[8];
+    for (int i = 0; i < N; ++i) {
+      if (at[i] < 0) continue;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = Half2Of<O>::down(x[2 * j], x[2 * j + 1]);
-        reinterpret_cast<uint4*>(dst)[0] = make_uint4(o[0], o[1], o[2], o[3]);
-        reinterpret_cast<uint4*>(dst)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+      for (int w = 0; w < 2; ++w) {
+        const uint32_t uw[4] = {u[w][i].x, u[w][i].y, u[w][i].z, u[w][i].w};
+        float x[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if (FMT == GL_KV_INT4) {
+            x[j] = (float)((int)((uw[j >> 3] >> (4 * (j & 7))) & 15u) - zero[w][i]) * scale[w][i];
+          } else {
+            const uint32_t byte = (uw[j >> 2] >> (8 * (j & 3))) & 255u;
+            x[j] = (FMT == GL_KV_FP8 ? gl_e4m3_to_float(byte) : (float)(int8_t)byte) * scale[w][i];
+          }
+        }
+        O* dst = reinterpret_cast<O*>(p.out[w]) + ((int64_t)b * p.max_len * hkv + at[i]) * D + lane * 16;
+        if constexpr (sizeof(O) == 4) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) __stcs(reinterpret_cast<float4*>(dst) + j, make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]));
+        } else {
+          uint32_t o[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[j] = Half2Of<O>::down(x[2 * j], x[2 * j + 1]);
+          __stcs(reinterpret_cast<uint4*>(dst), make_uint4(o[0], o[1], o[2], o[3]));
+          __stcs(reinterpret_cast<uint4*>(dst) + 1, make_uint4(o[4], o[5], o[6], o[7]));
+        }
       }
     }
   }
 }
 
-template <typename T, int LPR>
-int launch_write(const WriteParams& p, int fmt, dim3 grid, cudaStream_t st) {
+template <typename T, int LPR, bool INTER>
+int launch_write_fmt(const WriteParams& p, int fmt, dim3 grid, cudaStream_t st) {
   switch (fmt) {
-    case GL_KV_FP8: GL_CUDA_CHECK(gl_launch_pdl(kv_write_kernel<T, LPR, GL_KV_FP8>, grid, dim3(256), 0, st, p)); break;
-    case GL_KV_INT8: GL_CUDA_CHECK(gl_launch_pdl(kv_write_kernel<T, LPR, GL_KV_INT8>, grid, dim3(256), 0, st, p)); break;
-    default: GL_CUDA_CHECK(gl_launch_pdl(kv_write_kernel<T, LPR, GL_KV_INT4>, grid, dim3(256), 0, st, p)); break;
+    case GL_KV_FP8: GL_CUDA_CHECK(gl_launch_pdl(kv_write_kernel<T, LPR, GL_KV_FP8, INTER>, grid, dim3(256), 0, st, p)); break;
+    case GL_KV_INT8: GL_CUDA_CHECK(gl_launch_pdl(kv_write_kernel<T, LPR, GL_KV_INT8, INTER>, grid, dim3(256), 0, st, p)); break;
+    default: GL_CUDA_CHECK(gl_launch_pdl(kv_write_kernel<T, LPR, GL_KV_INT4, INTER>, grid, dim3(256), 0, st, p)); break;
   }
   return GL_OK;
+}
+template <typename T, int LPR>
+int launch_write(const WriteParams& p, bool interleaved, int fmt, dim3 grid, cudaStream_t st) {
+  return interleaved ? launch_write_fmt<T, LPR, true>(p, fmt, grid, st) : launch_write_fmt<T, LPR, false>(p, fmt, grid, st);
 }
 template <int D, typename O>
 int launch_read(const ReadParams& p, int fmt, dim3 grid, cudaStream_t st) {
@@ -326,6 +412,7 @@ extern "C" int gl_kv_write(const gl_kv_args* a, void* stream) {
   if (a->rot_dim < 0 || a->rot_dim > a->head_dim || a->rot_dim % 16 != 0)
     GL_FAIL(GL_E_INVALID, "gl_kv_write: rot_dim %d must be a multiple of 16 up to head_dim", a->rot_dim);
   if (a->rot_dim > 0 && (!a->cos_sin || !a->positions || a->table_rows <= 0)) GL_FAIL(GL_E_INVALID, "gl_kv_write: the rotation needs positions and a cos / sin table");
+  if (a->rot_dim > 0 && ((uintptr_t)a->cos_sin & 15)) GL_FAIL(GL_E_INVALID, "gl_kv_write: the cos / sin table must be 16-byte aligned");
   if ((a->q_norm || a->k_norm) && a->norm_dtype != GL_FP32 && a->norm_dtype != GL_FP16 && a->norm_dtype != GL_BF16)
     GL_FAIL(GL_E_INVALID, "gl_kv_write: norm weights of dtype %d", a->norm_dtype);
   WriteParams p;
@@ -336,16 +423,17 @@ extern "C" int gl_kv_write(const gl_kv_args* a, void* stream) {
   p.zeros[0] = a->k_zeros; p.zeros[1] = a->v_zeros;
   p.scales[0] = a->k_scales; p.scales[1] = a->v_scales;
   p.q_sn = a->q_stride_n; p.q_sh = a->q_stride_h; p.k_sn = a->k_stride_n; p.k_sh = a->k_stride_h; p.v_sn = a->v_stride_n; p.v_sh = a->v_stride_h;
-  p.hq = a->n_q_heads; p.rot = a->rot_dim; p.interleaved = a->interleaved; p.table_rows = a->table_rows; p.norm_dtype = a->norm_dtype;
+  p.hq = a->n_q_heads; p.rot = a->rot_dim; p.table_rows = a->table_rows; p.norm_dtype = a->norm_dtype;
   p.eps = a->eps;
   // few tokens: their heads are spread over blocks until every SM has a few; many: one block walks a token's heads
   const int lpr = a->head_dim / 8, groups = 256 / lpr;
-  const int64_t slices = gl_cdiv((a->q ? a->n_q_heads : 0) + 2 * a->n_kv_heads, groups), want = gl_cdiv((int64_t)gl_num_sms() * 8, a->n_tokens);
-  const dim3 grid((unsigned)a->n_tokens, (unsigned)(slices < want ? slices : want));
+  const int64_t slices = gl_cdiv(a->q ? a->n_q_heads : 0, groups) + gl_cdiv(2 * a->n_kv_heads, groups), want = gl_cdiv((int64_t)gl_num_sms() * 8, a->n_tokens);
+  const int64_t walk = (int64_t)gl_num_sms() * 12;
+  const dim3 grid((unsigned)(a->n_tokens < walk ? a->n_tokens : walk), (unsigned)(slices < want ? slices : want));
   cudaStream_t st = (cudaStream_t)stream;
   if (a->x_dtype == GL_BF16)
-    return lpr == 16 ? launch_write<__nv_bfloat16, 16>(p, a->format, grid, st) : launch_write<__nv_bfloat16, 8>(p, a->format, grid, st);
-  return lpr == 16 ? launch_write<__half, 16>(p, a->format, grid, st) : launch_write<__half, 8>(p, a->format, grid, st);
+    return lpr == 16 ? launch_write<__nv_bfloat16, 16>(p, a->interleaved != 0, a->format, grid, st) : launch_write<__nv_bfloat16, 8>(p, a->interleaved != 0, a->format, grid, st);
+  return lpr == 16 ? launch_write<__half, 16>(p, a->interleaved != 0, a->format, grid, st) : launch_write<__half, 8>(p, a->interleaved != 0, a->format, grid, st);
 }
 
 extern "C" int gl_kv_read(const gl_kv_args* a, void* stream) {
@@ -353,16 +441,17 @@ extern "C" int gl_kv_read(const gl_kv_args* a, void* stream) {
   if (a->x_dtype != GL_FP16 && a->x_dtype != GL_BF16 && a->x_dtype != GL_FP32) GL_FAIL(GL_E_UNSUPPORTED, "gl_kv_read: output dtype %d", a->x_dtype);
   if (a->batch == 0 || a->max_len == 0) return GL_OK;
   if (!a->out || !a->out_v || (((uintptr_t)a->out | (uintptr_t)a->out_v) & 15)) GL_FAIL(GL_E_INVALID, "gl_kv_read: null or misaligned output");
-  if (a->n_kv_heads > 65535) GL_FAIL(GL_E_UNSUPPORTED, "gl_kv_read: %d heads", a->n_kv_heads);
+  if ((int64_t)a->max_len * a->n_kv_heads > 0xffffffffll) GL_FAIL(GL_E_UNSUPPORTED, "gl_kv_read: %d tokens of %d heads", a->max_len, a->n_kv_heads);
   ReadParams p;
   p.kb = gl_kv_batch(a);
   p.codes[0] = (const uint8_t*)a->k_codes; p.codes[1] = (const uint8_t*)a->v_codes;
   p.zeros[0] = a->k_zeros; p.zeros[1] = a->v_zeros;
   p.scales[0] = a->k_scales; p.scales[1] = a->v_scales;
   p.out[0] = a->out; p.out[1] = a->out_v;
-  p.max_len = a->max_len; p.out_dtype = a->x_dtype;
+  p.max_len = a->max_len;
+  p.heads_shift = (a->n_kv_heads & (a->n_kv_heads - 1)) == 0 ? __builtin_ctz((unsigned)a->n_kv_heads) : -1;
   const int rows = 256 / (a->head_dim / 16);
-  const dim3 grid((unsigned)gl_cdiv(a->max_len, rows), (unsigned)a->n_kv_heads, (unsigned)(a->batch < 65535 ? a->batch : 65535));
+  const dim3 grid((unsigned)gl_cdiv((int64_t)a->max_len * a->n_kv_heads, rows * 2), (unsigned)(a->batch < 65535 ? a->batch : 65535));
   cudaStream_t st = (cudaStream_t)stream;
   if (a->head_dim == 128) {
     if (a->x_dtype == GL_BF16) return launch_read<128, __nv_bfloat16>(p, a->format, grid, st);

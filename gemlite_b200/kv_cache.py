@@ -244,6 +244,8 @@ class QuantizedKVCache:
             if positions.dtype != torch.int32:
                 raise ValueError("positions must be int32 or int64, got %s" % positions.dtype)
             positions = positions.contiguous()
+            if cos_sin.data_ptr() & 15:
+                cos_sin = cos_sin.clone()
             a.cos_sin, a.positions, a.rot_dim, a.table_rows = cos_sin.data_ptr(), positions.data_ptr(), cos_sin.shape[1], cos_sin.shape[0]
             if a.table_rows == 0:
                 raise ValueError("cos_sin has no rows")

@@ -332,7 +332,7 @@ typedef struct gl_kv_args {
   void*          out_v;         /* read: values */
   const void*    q_norm;        /* write: weights of the head norms [head_dim] (norm_dtype), or NULL */
   const void*    k_norm;
-  const float*   cos_sin;       /* write: [table_rows, rot_dim], cosines then sines, or NULL */
+  const float*   cos_sin;       /* write: [table_rows, rot_dim], cosines then sines, 16-byte aligned, or NULL */
   const int32_t* positions;     /* write: [n_tokens], row of cos_sin */
   const uint8_t* mask;          /* attend: [n_tokens, mask_cols], rows mask_stride apart, or NULL */
   void*          workspace;     /* attend: gl_kv_attend_workspace_bytes(), 16-byte aligned, any content */
