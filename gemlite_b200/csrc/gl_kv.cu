@@ -3,7 +3,7 @@
 // Both kernels move bytes: every operand is read once with 16-byte loads, every output written once.  A row (one token's
 // head) is spread over head_dim / 8 lanes of 8 channels each, so that norms and maxima are three or four shuffles and the
 // rotation's partner channel is one.
-#include "gl_kv.cuh"
+#include "gl_kv_attend.cuh"
 
 int gl_kv_check(const char* fn, const gl_kv_args* a) {
   if (a == nullptr) GL_FAIL(GL_E_INVALID, "%s: null argument struct", fn);
@@ -301,77 +301,83 @@ struct ReadParams {
   int32_t max_len, heads_shift;
 };
 
-// One lane per 16 channels of a row, keys and values of the same slot by the same lane.  A block takes whole tokens (all heads of
-// one follow each other in the output) and several rows per lane, whose loads are issued together.
+// One lane per 8 channels, so that a warp's stores are whole lines of the output; a block takes whole tokens (all heads of one
+// follow each other there).  Its rows' slots are looked up once, by one thread each, and every lane has the loads of eight rows, keys
+// and values, in flight.  Codes become fp16 numbers two at a time, exactly, and are scaled in fp32.
 template <int D, int FMT, typename O>
 __global__ void __launch_bounds__(256) kv_read_kernel(const ReadParams p) {
-  constexpr int LPR = D / 16, ROWS = 256 / LPR, N = 2;
-  const int lane = threadIdx.x % LPR, hkv = p.kb.hkv;
-  const int64_t row0 = (int64_t)blockIdx.x * (ROWS * N) + threadIdx.x / LPR;
+  constexpr int RB = FMT == GL_KV_INT4 ? D / 2 : D, LPR = D / 8, GROUPS = 256 / LPR, N = 8, ROWS = GROUPS * N;
+  __shared__ int64_t slots[ROWS];              // -1: zeros
+  const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR, hkv = p.kb.hkv;
+  const int64_t row0 = (int64_t)blockIdx.x * ROWS, end = (int64_t)p.max_len * hkv;
   gl_launch_dependents();
   gl_grid_dependency_wait();
   for (int b = blockIdx.y; b < p.kb.batch; b += gridDim.y) {
-    const int len = p.kb.lens[b];
-    int64_t slot[N], at[N];
+    for (int i = threadIdx.x; i < ROWS; i += 256) {
+      const int64_t row = row0 + i;
+      const uint32_t t = p.heads_shift >= 0 ? (uint32_t)(row >> p.heads_shift) : (uint32_t)((uint64_t)row / (uint32_t)hkv);
+      slots[i] = row < end && (int64_t)t < p.kb.lens[b] ? kv_slot(p.kb, b, (int)(row - (int64_t)t * hkv), t) : -1;
+    }
+    __syncthreads();
+    uint2 u[2][N];
+    float scale[2][N];
+    uint32_t zero[2][N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int64_t row = row0 + i * ROWS;
-      const uint32_t t = p.heads_shift >= 0 ? (uint32_t)(row >> p.heads_shift) : (uint32_t)((uint64_t)row / (uint32_t)hkv);
-      const int h = (int)(row - (int64_t)t * hkv);
-      at[i] = t < (uint32_t)p.max_len ? row : -1;
-      slot[i] = at[i] >= 0 && (int64_t)t < len ? kv_slot(p.kb, b, h, t) : -1;
-    }
-    uint4 u[2][N];
-    float scale[2][N];
-    int zero[2][N];
-#pragma unroll
-    for (int i = 0; i < N; ++i)
+      const int64_t slot = slots[i * GROUPS + group];
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        u[w][i] = make_uint4(0, 0, 0, 0);
+        u[w][i] = make_uint2(0, 0);
         scale[w][i] = 0.f;
         zero[w][i] = 0;
-        if (slot[i] >= 0) {
-          scale[w][i] = p.scales[w][slot[i]];
-          if (FMT == GL_KV_INT4) {
-            const uint2 x = *reinterpret_cast<const uint2*>(p.codes[w] + slot[i] * (D / 2) + lane * 8);
-            u[w][i].x = x.x;
-            u[w][i].y = x.y;
-            zero[w][i] = p.zeros[w][slot[i]];
+        if (slot >= 0) {
+          if constexpr (FMT == GL_KV_INT4) {
+            u[w][i].x = __ldcs(reinterpret_cast<const uint32_t*>(p.codes[w] + slot * RB) + lane);
+            zero[w][i] = p.zeros[w][slot];
           } else {
-            u[w][i] = *reinterpret_cast<const uint4*>(p.codes[w] + slot[i] * D + lane * 16);
+            u[w][i] = __ldcs(reinterpret_cast<const uint2*>(p.codes[w] + slot * RB) + lane);
           }
-        }
-      }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (at[i] < 0) continue;
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const uint32_t uw[4] = {u[w][i].x, u[w][i].y, u[w][i].z, u[w][i].w};
-        float x[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          if (FMT == GL_KV_INT4) {
-            x[j] = (float)((int)((uw[j >> 3] >> (4 * (j & 7))) & 15u) - zero[w][i]) * scale[w][i];
-          } else {
-            const uint32_t byte = (uw[j >> 2] >> (8 * (j & 3))) & 255u;
-            x[j] = (FMT == GL_KV_FP8 ? gl_e4m3_to_float(byte) : (float)(int8_t)byte) * scale[w][i];
-          }
-        }
-        O* dst = reinterpret_cast<O*>(p.out[w]) + ((int64_t)b * p.max_len * hkv + at[i]) * D + lane * 16;
-        if constexpr (sizeof(O) == 4) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) __stcs(reinterpret_cast<float4*>(dst) + j, make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]));
-        } else {
-          uint32_t o[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) o[j] = Half2Of<O>::down(x[2 * j], x[2 * j + 1]);
-          __stcs(reinterpret_cast<uint4*>(dst), make_uint4(o[0], o[1], o[2], o[3]));
-          __stcs(reinterpret_cast<uint4*>(dst) + 1, make_uint4(o[4], o[5], o[6], o[7]));
+          scale[w][i] = p.scales[w][slot];
         }
       }
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int64_t row = row0 + i * GROUPS + group;
+      if (row >= end) continue;
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        uint32_t h[4];
+        if constexpr (FMT == GL_KV_INT4) {
+          const uint32_t z = (0x6400u + zero[w][i]) * 0x10001u, c = u[w][i].x;
+          uint32_t n[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) n[k] = kv_nibbles(c >> (4 * k), z);      // channels (k, k + 4)
+          h[0] = __byte_perm(n[0], n[1], 0x5410);
+          h[1] = __byte_perm(n[2], n[3], 0x5410);
+          h[2] = __byte_perm(n[0], n[1], 0x7632);
+          h[3] = __byte_perm(n[2], n[3], 0x7632);
+        } else {
+          kv_bytes<FMT>(u[w][i].x, h[0], h[1]);
+          kv_bytes<FMT>(u[w][i].y, h[2], h[3]);
+        }
+        float2 f[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          f[k] = __half22float2(*reinterpret_cast<const __half2*>(&h[k]));
+          f[k].x *= scale[w][i];
+          f[k].y *= scale[w][i];
+        }
+        O* dst = reinterpret_cast<O*>(p.out[w]) + ((int64_t)b * end + row) * D + lane * 8;
+        if constexpr (sizeof(O) == 4) {
+          __stcs(reinterpret_cast<float4*>(dst), make_float4(f[0].x, f[0].y, f[1].x, f[1].y));
+          __stcs(reinterpret_cast<float4*>(dst) + 1, make_float4(f[2].x, f[2].y, f[3].x, f[3].y));
+        } else {
+          __stcs(reinterpret_cast<uint4*>(dst), make_uint4(Half2Of<O>::down(f[0].x, f[0].y), Half2Of<O>::down(f[1].x, f[1].y), Half2Of<O>::down(f[2].x, f[2].y), Half2Of<O>::down(f[3].x, f[3].y)));
+        }
+      }
+    }
+    __syncthreads();                           // the slots may be overwritten
   }
 }
 
@@ -450,8 +456,8 @@ extern "C" int gl_kv_read(const gl_kv_args* a, void* stream) {
   p.out[0] = a->out; p.out[1] = a->out_v;
   p.max_len = a->max_len;
   p.heads_shift = (a->n_kv_heads & (a->n_kv_heads - 1)) == 0 ? __builtin_ctz((unsigned)a->n_kv_heads) : -1;
-  const int rows = 256 / (a->head_dim / 16);
-  const dim3 grid((unsigned)gl_cdiv((int64_t)a->max_len * a->n_kv_heads, rows * 2), (unsigned)(a->batch < 65535 ? a->batch : 65535));
+  const int rows = 256 / (a->head_dim / 8) * 8;
+  const dim3 grid((unsigned)gl_cdiv((int64_t)a->max_len * a->n_kv_heads, rows), (unsigned)(a->batch < 65535 ? a->batch : 65535));
   cudaStream_t st = (cudaStream_t)stream;
   if (a->head_dim == 128) {
     if (a->x_dtype == GL_BF16) return launch_read<128, __nv_bfloat16>(p, a->format, grid, st);
