@@ -27,10 +27,11 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .dtypes import TORCH_TO_DTYPE, DType
+from .dtypes import DType
 
 KV_FORMATS = {"fp8": 0, "int8": 1, "int4": 2}
 _DTYPE_CODES = {torch.float16: DType.FP16.value, torch.bfloat16: DType.BF16.value, torch.float32: DType.FP32.value}
+_HALF_CODES = {torch.float16: DType.FP16.value, torch.bfloat16: DType.BF16.value}
 _INT32_MAX = 2 ** 31 - 1
 
 
@@ -75,6 +76,7 @@ class KVBatch:
         for t in (ctx_lens, q_offsets):
             if t is not None and t.device != page_table.device:
                 raise ValueError("page_table, ctx_lens and q_offsets must be on one device")
+        self.device, self.shape, self.table_stride = page_table.device, tuple(page_table.shape), page_table.stride(0)
         self.max_len = None if max_len is None else max(0, min(int(max_len), _INT32_MAX))
         self.max_new = None if max_new is None else max(0, min(int(max_new), _INT32_MAX))
 
@@ -137,54 +139,60 @@ class QuantizedKVCache:
         a.n_kv_heads, a.head_dim = self.n_kv_heads, self.head_dim
         self._args = bytes(a)
 
-    # -- argument plumbing ---------------------------------------------------------------------------------------------
+    # -- argument plumbing (a decode step makes these calls once per layer: what they cost the host counts) ----------------------
     def _on_device(self, t, what):
-        _lib.require_cuda(t, what)
-        if t.device != self.device:
+        if not isinstance(t, Tensor) or t.device != self.device:
+            _lib.require_cuda(t, what)
             raise ValueError("%s is on %s, the cache on %s" % (what, t.device, self.device))
         return t
 
     def _rows(self, x, what, heads=None):
-        """(tensor, token stride, head stride) of a [tokens, heads, head_dim] operand; copied only where the kernels could not
-        read it with 16-byte loads."""
+        """(tensor, address, token stride, head stride, tokens, heads) of a [tokens, heads, head_dim] operand; copied only
+        where the kernels could not read it with 16-byte loads."""
         self._on_device(x, what)
-        if x.dtype not in (torch.float16, torch.bfloat16):
+        if x.dtype not in _HALF_CODES:
             raise NotImplementedError("%s must be float16 or bfloat16, got %s" % (what, x.dtype))
-        if x.dim() != 3 or x.shape[2] != self.head_dim or (heads is not None and x.shape[1] != heads):
-            raise ValueError("%s must be [tokens, %s, %d], got %s" % (what, "heads" if heads is None else heads, self.head_dim, tuple(x.shape)))
-        n, h, _ = x.shape
+        shape = x.shape
+        if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
+            raise ValueError("%s must be [tokens, %s, %d], got %s" % (what, "heads" if heads is None else heads, self.head_dim, tuple(shape)))
+        n, h, _ = shape
         sn, sh, sd = x.stride()
         if n <= 1:
             sn = 0
         if h == 1:
             sh = 0
-        if sd != 1 or (sn | sh) & 7 or x.data_ptr() & 15:
+        at = x.data_ptr()
+        if sd != 1 or (sn | sh) & 7 or at & 15:
             x = x.clone(memory_format=torch.contiguous_format)
-            sn, sh = h * self.head_dim, self.head_dim
-        return x, sn, sh
+            at, sn, sh = x.data_ptr(), h * self.head_dim, self.head_dim
+        return x, at, sn, sh, n, h
 
     def _batch_args(self, batch, n):
         a = _lib.GLKvArgs.from_buffer_copy(self._args)
-        table = batch.page_table
-        if table.device != self.device:
-            raise ValueError("the batch is on %s, the cache on %s" % (table.device, self.device))
-        B, P = table.shape
-        a.page_table, a.page_table_stride, a.lens = table.data_ptr(), table.stride(0), batch.ctx_lens.data_ptr()
+        if batch.device != self.device:
+            raise ValueError("the batch is on %s, the cache on %s" % (batch.device, self.device))
+        B, P = batch.shape
+        a.page_table, a.page_table_stride, a.lens = batch.page_table.data_ptr(), batch.table_stride, batch.ctx_lens.data_ptr()
         if batch.q_offsets is not None:
             a.q_offsets = batch.q_offsets.data_ptr()
-        elif B > 0 and n % B != 0:
-            raise ValueError("%d rows do not divide evenly over %d sequences; give the batch q_offsets" % (n, B))
+            a.max_new = n if batch.max_new is None else batch.max_new
+        elif B > 0:
+            if n % B != 0:
+                raise ValueError("%d rows do not divide evenly over %d sequences; give the batch q_offsets" % (n, B))
+            a.max_new = n // B if batch.max_new is None else batch.max_new
         a.batch, a.max_pages, a.n_tokens = B, P, n
         a.max_len = min(P * self.page_size, _INT32_MAX) if batch.max_len is None else batch.max_len
-        if batch.max_new is not None:
-            a.max_new = batch.max_new
-        else:
-            a.max_new = n if batch.q_offsets is not None or B == 0 else n // B
         return a
 
     def _call(self, fn, a):
-        with torch.cuda.device(self.device):
-            _lib.check(fn(ctypes.byref(a), _lib.current_stream_ptr(self.device)))
+        index = self.device.index
+        if torch._C._cuda_getDevice() == index:
+            status = fn(ctypes.byref(a), _lib.current_stream_ptr(self.device))
+        else:
+            with torch.cuda.device(index):
+                status = fn(ctypes.byref(a), _lib.current_stream_ptr(self.device))
+        if status:
+            _lib.check(status)
 
     # -- operators -----------------------------------------------------------------------------------------------------
     def write(self, q: Optional[Tensor], k: Tensor, v: Tensor, batch: KVBatch, positions: Optional[Tensor] = None,
@@ -202,21 +210,21 @@ class QuantizedKVCache:
         scale NaN.  A position outside the table gives NaN queries and such a key row.  Tokens whose page does not exist are
         dropped.  A page must not be written for two sequences in one call.  Rows of the result that belong to no
         sequence are not written."""
-        k, ksn, ksh = self._rows(k, "k", self.n_kv_heads)
-        v, vsn, vsh = self._rows(v, "v", self.n_kv_heads)
-        n = k.shape[0]
-        if v.shape[0] != n or v.dtype != k.dtype:
+        k, k_at, ksn, ksh, n, _ = self._rows(k, "k", self.n_kv_heads)
+        v, v_at, vsn, vsh, vn, _ = self._rows(v, "v", self.n_kv_heads)
+        dtype = k.dtype
+        if vn != n or v.dtype != dtype:
             raise ValueError("k and v must have the same tokens and dtype")
         a = self._batch_args(batch, n)
-        a.k, a.k_stride_n, a.k_stride_h, a.v, a.v_stride_n, a.v_stride_h = k.data_ptr(), ksn, ksh, v.data_ptr(), vsn, vsh
-        a.x_dtype = _DTYPE_CODES[k.dtype]
+        a.k, a.k_stride_n, a.k_stride_h, a.v, a.v_stride_n, a.v_stride_h = k_at, ksn, ksh, v_at, vsn, vsh
+        a.x_dtype = _HALF_CODES[dtype]
         out = None
         if q is not None:
-            q, qsn, qsh = self._rows(q, "q")
-            if q.shape[0] != n or q.dtype != k.dtype:
+            q, q_at, qsn, qsh, qn, qh = self._rows(q, "q")
+            if qn != n or q.dtype != dtype:
                 raise ValueError("q and k must have the same tokens and dtype")
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            a.q, a.q_stride_n, a.q_stride_h, a.n_q_heads, a.out = q.data_ptr(), qsn, qsh, q.shape[1], out.data_ptr()
+            out = torch.empty((n, qh, self.head_dim), dtype=dtype, device=self.device)
+            a.q, a.q_stride_n, a.q_stride_h, a.n_q_heads, a.out = q_at, qsn, qsh, qh, out.data_ptr()
         keep = []
         for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
             if w is not None:
@@ -282,8 +290,7 @@ class QuantizedKVCache:
         new tokens up to the query's own (single tokens, prompt chunks).  A row that sees nothing gives zeros; what a row does not
         see has no influence on it, whatever those slots hold.  scale defaults to 1 / sqrt(head_dim).
         Result like q (contiguous); rows that belong to no sequence are not written."""
-        q, sn, sh = self._rows(q, "q")
-        n, h, _ = q.shape
+        q, at, sn, sh, n, h = self._rows(q, "q")
         if h == 0 or h % self.n_kv_heads != 0:
             raise ValueError("%d query heads do not divide over %d kv heads" % (h, self.n_kv_heads))
         if out is None:
@@ -293,7 +300,7 @@ class QuantizedKVCache:
             if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() & 15:
                 raise ValueError("out must be a contiguous, 16-byte aligned %s tensor of shape %s" % (q.dtype, tuple(q.shape)))
         a = self._batch_args(batch, n)
-        a.q, a.q_stride_n, a.q_stride_h, a.n_q_heads, a.out, a.x_dtype = q.data_ptr(), sn, sh, h, out.data_ptr(), _DTYPE_CODES[q.dtype]
+        a.q, a.q_stride_n, a.q_stride_h, a.n_q_heads, a.out, a.x_dtype = at, sn, sh, h, out.data_ptr(), _HALF_CODES[q.dtype]
         a.softmax_scale = 1.0 / math.sqrt(self.head_dim) if scale is None else scale
         a.kernel_override = kernel_override
         if mask is not None:
@@ -308,10 +315,19 @@ class QuantizedKVCache:
         if n == 0 or a.batch == 0:
             return out
         L = _lib.lib()
-        with torch.cuda.device(self.device):
-            need = L.gl_kv_attend_workspace_bytes(ctypes.byref(a))
-            if need:
-                ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-                a.workspace, a.workspace_bytes = ws.data_ptr(), need
-            _lib.check(L.gl_kv_attend(ctypes.byref(a), _lib.current_stream_ptr(self.device)))
+        if torch._C._cuda_getDevice() == self.device.index:
+            self._attend(L, a)
+        else:
+            with torch.cuda.device(self.device.index):
+                self._attend(L, a)
         return out
+
+    def _attend(self, L, a):
+        at = ctypes.byref(a)
+        need = L.gl_kv_attend_workspace_bytes(at)
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        status = L.gl_kv_attend(at, _lib.current_stream_ptr(self.device))
+        if status:
+            _lib.check(status)

@@ -9,8 +9,9 @@ The reference has no multi-GPU code: under vLLM the host shards the weights and 
   bias is added on rank 0 only, before the reduction.
 
 `LlamaLinears` strings the seven linears of one Llama decoder layer together (fused qkv, o, fused gate/up, down)
-with the two all-reduces, which is the communication pattern of a tensor-parallel decoder step; attention
-itself and the norms are not part of the low-bit matmul path and are not modelled.
+with the two all-reduces, which is the communication pattern of a tensor-parallel decoder step.  Given a quantised cache
+(`kv_cache.QuantizedKVCache` of the rank's kv heads) the step includes the attention between qkv and o; the layer norms and
+residuals are not part of the low-bit path and are not modelled.
 """
 import ctypes
 
@@ -193,6 +194,7 @@ class LlamaLinears(torch.nn.Module):
         self.q_local = n_heads * head_dim // world
         self.kv_local = n_kv_heads * head_dim // world
         self.inter_local = intermediate // world
+        self.head_dim = head_dim
         gen_dev = torch.device(device)
         g = torch.Generator(device=gen_dev).manual_seed(seed)   # same seed on every rank: all ranks shard the same matrices
 
@@ -214,9 +216,19 @@ class LlamaLinears(torch.nn.Module):
         self.gate_up = col(w(intermediate, hidden), w(intermediate, hidden))
         self.down = build_a16w4_tp_linear(w(hidden, intermediate), None, "row", world, rank, device, dtype, 4, group_size, comm)
 
-    def forward(self, x):
+    def forward(self, x, cache=None, batch=None, mask=None, **write):
+        """x [tokens, hidden].  With a `QuantizedKVCache` of the rank's kv heads and a `KVBatch`, the attention of the local heads runs over
+        the cache: keys and values are written behind each sequence's cached tokens (`write`: positions, cos_sin, q_norm,
+        k_norm, eps, interleaved as in `QuantizedKVCache.write`), then every token attends (`mask`: a tree of drafts).  Without
+        a cache a slice of the projection stands in for the attention's output: the linears alone."""
         qkv = self.qkv(x)
-        attn = qkv[..., : self.q_local].contiguous()          # stand-in for the attention output of the local heads
+        if cache is None:
+            attn = qkv[..., : self.q_local].contiguous()      # stand-in for the attention output of the local heads
+        else:
+            d, flat = self.head_dim, qkv.view(-1, qkv.shape[-1])
+            q, k, v = (t.view(flat.shape[0], -1, d) for t in flat.split([self.q_local, self.kv_local, self.kv_local], 1))
+            q = cache.write(q, k, v, batch, **write)
+            attn = cache.attend(q, batch, mask=mask).view(*qkv.shape[:-1], self.q_local)
         h = self.o(attn)
         gu = self.gate_up(h)
         return self.down(silu_mul(gu))

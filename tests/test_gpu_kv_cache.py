@@ -381,6 +381,32 @@ def test_prompt_draft_accept_decode(lib, fmt):
         assert torch.equal(x[:, :55], y[:, :55])
 
 
+def test_decoder_layer_linears_with_the_cache(lib):
+    """tp.LlamaLinears: without a cache as before; with one, the output projection's input is the attention of the formula."""
+    from gemlite_b200 import KVBatch, rotary_table, tp
+    hidden, hq, hkv, d = 512, 8, 2, 64
+    layer = tp.LlamaLinears(hidden, 1024, hq, hkv, d, 1, 0, DEV, seed=3)
+    cache, table = make_cache([40, 9], hkv, d, "fp8", 16, seed=21)
+    x = _randn(1, 5, hidden)
+    seen = []
+    layer.o.register_forward_pre_hook(lambda m, a: seen.append(a[0].clone()))
+    layer.qkv.register_forward_hook(lambda m, a, y: seen.append(y.clone()))
+    layer(x)
+    assert torch.equal(seen[1], seen[0][:, :hq * d])
+    seen.clear()
+    batch, cs = KVBatch(table, _i32([36, 8]), _i32([0, 4, 5])), rotary_table(64, d, device=DEV)
+    pos = torch.tensor([36, 37, 38, 39, 8], device=DEV)
+    y = layer(x, cache, batch, positions=pos, cos_sin=cs)
+    assert y.shape == x.shape and bool(y.isfinite().all())
+    qkv, attn = seen
+    q = qkv[:, :hq * d].view(5, hq, d)
+    q64 = rotate64(q.double(), cs, pos, False)
+    tol = torch.finfo(q.dtype).eps / 2 * q64.abs() + 16 * 2.0 ** -24 * q64.abs().amax(-1, keepdim=True)
+    rotated = cache.write(q, qkv[:, hq * d:(hq + hkv) * d].view(5, hkv, d), qkv[:, (hq + hkv) * d:].view(5, hkv, d), batch, positions=pos, cos_sin=cs)
+    assert bool(((rotated.double() - q64).abs() <= tol).all())
+    _check_attend(cache, table, [36, 8], [4, 1], rotated, None, attn.view(5, hq, d))
+
+
 def test_graph_capture_streams_and_repeats(lib):
     """A captured step replays with what the tensors hold then; two graphs and a side stream do not share scratch; the same
     call gives the same bits."""

@@ -43,16 +43,18 @@ def test_unsupported_and_call_specific(lib):
         assert f(ctypes.byref(_args(x_dtype=4)), None) == _lib.GL_E_UNSUPPORTED
         assert f(None, None) == _lib.GL_E_INVALID
         assert f(ctypes.byref(_args(batch=0, max_len=0, n_tokens=0)), None) == _lib.GL_OK
-    for bad in ({"rot_dim": 24}, {"rot_dim": 144}, {"rot_dim": 64}, {"k": None}, {"q_stride_n": 4}, {"v": (1 << 20) + 2},
+    for bad in ({"rot_dim": 24}, {"rot_dim": 144}, {"rot_dim": 64}, {"rot_dim": 64, "cos_sin": (1 << 20) + 4, "positions": 1 << 20, "table_rows": 4}, {"k": None}, {"q_stride_n": 4}, {"v": (1 << 20) + 2},
                 {"q_norm": 1 << 20, "norm_dtype": 4}, {"n_q_heads": 0}):
         assert lib.gl_kv_write(ctypes.byref(_args(**bad)), None) == _lib.GL_E_INVALID, bad
     for bad in ({"n_q_heads": 3}, {"n_q_heads": 0}, {"q": None}, {"q_stride_h": 12}, {"mask": 1 << 20, "mask_cols": -1}, {"kernel_override": 3}):
         assert lib.gl_kv_attend(ctypes.byref(_args(**bad)), None) == _lib.GL_E_INVALID, bad
     assert lib.gl_kv_attend(ctypes.byref(_args(n_q_heads=1 << 16, n_kv_heads=1, n_tokens=1 << 16)), None) == _lib.GL_E_UNSUPPORTED
     assert lib.gl_kv_attend(ctypes.byref(_args(max_pages=1 << 28)), None) == _lib.GL_E_UNSUPPORTED
+    for fn in ("gl_kv_write", "gl_kv_read", "gl_kv_attend"):       # slots are 32-bit numbers
+        assert getattr(lib, fn)(ctypes.byref(_args(num_pages=1 << 26, page_size=64)), None) == _lib.GL_E_UNSUPPORTED
     long = _args(max_pages=1 << 12, max_len=1 << 16)
     need = lib.gl_kv_attend_workspace_bytes(ctypes.byref(long))
-    assert need > 0 and need % (2 * 4 * (128 * 4 + 8)) == 0
+    assert need > 0 and need % 16 == 0
     assert lib.gl_kv_attend(ctypes.byref(long), None) == _lib.GL_E_WORKSPACE and str(need).encode() in lib.gl_last_error()
 
 
