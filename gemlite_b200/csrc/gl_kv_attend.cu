@@ -20,7 +20,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kTinyScale = 1e-30f;
 constexpr int kTile = 32;          // tokens that a warp takes at a time
 constexpr int kWarps = 4;
-constexpr int kStages = 2;
+constexpr int kStages = 3;
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) { return __byte_perm(a, b, s); }
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -56,10 +56,14 @@ template <int D, int FMT> struct Shape {
   static constexpr int LOOP = kWarps * kStages * STAGE;
 };
 
+// Thread blocks per SM: what shared memory (8-bit rows of 128) and registers without spills let in.  32 decoding sequences of
+// 64 / 8 heads of 128 in fp8: 99 us with two blocks and three stages, 105 us with three blocks and two.
+constexpr int kv_mma_blocks(int d, int fmt, int nr) { return d == 64 ? (nr == 1 ? 4 : 3) : nr == 1 && fmt == GL_KV_INT4 ? 3 : 2; }
+
 // Transposed products: S^T = K Q^T and O^T = V^T P^T, so that the tokens (keys) or the channels (values) are the 16 rows of the
 // MMA and 8 query rows its columns: a single token of a group of 8 heads fills them.  NR tiles of 8 query rows.
 template <int D, int FMT, int NR, typename T>
-__global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 3 : 2) kv_attend_mma_kernel(const KvAttendParams p) {
+__global__ void __launch_bounds__(kWarps * 32, kv_mma_blocks(D, FMT, NR)) kv_attend_mma_kernel(const KvAttendParams p) {
   using S = Shape<D, FMT>;
   constexpr int RB = S::RB, CPT = RB / 16, NT = D / 8, KS = D / 16, ROWS = 8 * NR;
   constexpr float kShift = 15.f;
@@ -624,7 +628,7 @@ int launch_all(const KvAttendParams& p, const gl_kv_args* a, const Plan& pl, cud
   return pl.rows == 8 ? launch_join<8, D, T>(p, pl, st) : launch_join<16, D, T>(p, pl, st);
 }
 
-// Few rows per kv head: the mma.sync kernel, which holds 8 or 16 rows in registers (three or two blocks per SM); more: the
+// Few rows per kv head: the mma.sync kernel, which holds 8 or 16 rows in registers; more: the
 // tcgen05 kernel with 256 (one per SM).
 Plan plan_of(const gl_kv_args* a) {
   Plan pl;
@@ -638,7 +642,7 @@ Plan plan_of(const gl_kv_args* a) {
   int64_t len = a->max_len < cap ? a->max_len : cap;
   if (len < 1) len = 1;
   const int64_t units = (int64_t)a->batch * a->n_kv_heads * gl_cdiv(max_rows, pl.rows), work = units * gl_cdiv(len, kKvTile);
-  int64_t most = (int64_t)gl_num_sms() * (tc ? 1 : pl.rows == 8 ? 3 : 2);
+  int64_t most = (int64_t)gl_num_sms() * (tc ? 1 : kv_mma_blocks(a->head_dim, a->format, pl.rows / 8));
   if (most > kJoinMax) most = kJoinMax;
   pl.blocks = (int)(work < most ? work : most);
   // units cut into many parts are joined by a block per row, others by one per 8 rows
