@@ -12,7 +12,6 @@
 // leaves the fp16 format 39 binary orders below the largest weight before a weight is lost.
 #include "gl_kv_attend.cuh"
 #include <mutex>
-#include <vector>
 
 namespace {
 
@@ -672,17 +671,18 @@ uint64_t workspace_of(const gl_kv_args* a, const Plan& pl) {
 }  // namespace
 
 int kv_allow_smem(const void* kernel, int bytes) {
-  // remembered per device and kernel; a kernel that is not found twice at the same time is set twice, which does no harm
+  // remembered per kernel and device; without room left the attribute is set every time, which does no harm
   struct Entry { const void* kernel; int dev; };
+  static Entry done[512];
+  static int count = 0;
   static std::mutex mu;
-  static std::vector<Entry> done;
   int dev = 0;
   GL_CUDA_CHECK(cudaGetDevice(&dev));
   std::lock_guard<std::mutex> lk(mu);
-  for (const Entry& e : done)
-    if (e.kernel == kernel && e.dev == dev) return GL_OK;
+  for (int i = 0; i < count; ++i)
+    if (done[i].kernel == kernel && done[i].dev == dev) return GL_OK;
   GL_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  done.push_back({kernel, dev});
+  if (count < 512) done[count++] = Entry{kernel, dev};
   return GL_OK;
 }
 

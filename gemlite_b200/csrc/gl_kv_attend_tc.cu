@@ -6,8 +6,8 @@
 //   K'[p] = fp16(kq[p] ks[p] / KS),  V'[p] = fp16(vq[p] vs[p] / VS)          (one rounding of 2^-11 each; codes are exact)
 //   S = q K'^T,  P = 2^(a S + log2 VS - M + 7),  O += P V',  l += sum P / VS,  a = log2(e) c KS (times q's power of two)
 // and a score costs one multiply-add, one exponential, one maximum and one addition.  None of these numbers is a subnormal
-// fp16 number as long as the scales lie within 2^12 of each other, so the choice of KS and VS changes no bit.  Where scales
-// lie further apart, and where tiles hold new tokens under a mask (a token that a row does not see must not round what it
+// fp16 number as long as the scales lie near each other (kSpread, kSpreadV), so the choice of KS and VS changes no bit.  Where
+// they lie further apart, and where tiles hold new tokens under a mask (a token that a row does not see must not round what it
 // sees), K' or V' stay the codes, and ks[p], or log2 vs[p] and 1 / vs[p], go to the scores, as in the other kernel.
 // M is a maximum of the exponents that lags: it is raised, and O and l are scaled, only when a row's new maximum is more than
 // 2^8 above it (P stays below 2^15 then, fp16's range, and keeps 31 binary orders below M).
@@ -69,9 +69,13 @@ __device__ __forceinline__ int pow2_above(uint32_t bits) {
 }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 
-// power of two that brings the largest code near the end of fp16's range
+// Keys: the power of two that brings the largest code near the end of fp16's range, so that scales 2^12 apart still give normal
+// fp16 numbers.  Values: none.  It would come out of the weights' range: P holds p VS, and tiles whose scales are not folded hold p vs,
+// so with room for the values weights of 2^-9 of the largest were subnormal numbers already (4 bits, a tree's draft tile beside its
+// cached ones).  Without it e4m3's subnormal codes allow scales 2^5 apart, whole numbers 2^12.
 template <int FMT> constexpr int kRoom = FMT == GL_KV_FP8 ? 7 : FMT == GL_KV_INT8 ? 8 : 12;
 constexpr int kSpread = 12;
+template <int FMT> constexpr int kSpreadV = FMT == GL_KV_FP8 ? 5 : 12;
 
 // scale ratio as two fp16 numbers (high, rest) of one value
 __device__ __forceinline__ uint32_t split_half(float r) {
@@ -242,8 +246,8 @@ __device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh
     const uint32_t bits = __float_as_uint(scale);
     const bool plain = bits - 1u < 0x7f7fffffu;                          // positive and finite
     const uint32_t hi = __reduce_max_sync(0xffffffffu, plain ? bits : 0u), lo = __reduce_min_sync(0xffffffffu, plain ? bits : 0x7f7fffffu);
-    const bool apart = (draft && p.mask != nullptr) || (int)(hi >> 23) - (int)(lo >> 23) >= kSpread;
-    const int e = apart ? 0 : pow2_above(hi) - kRoom<FMT>;
+    const bool apart = (draft && p.mask != nullptr) || (int)(hi >> 23) - (int)(lo >> 23) >= (values ? kSpreadV<FMT> : kSpread);
+    const int e = apart ? 0 : pow2_above(hi) - (values ? 0 : kRoom<FMT>);
     const bool number = fabsf(scale) < INFINITY, none = apart && scale < 1e-30f;
     const uint32_t valid = __ballot_sync(0xffffffffu, rows.slot != kNoSlot);
     // Values that are not numbers would reach every row through P V', so V' is 0 there, and the exponent is NaN, which only the

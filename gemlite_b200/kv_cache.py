@@ -223,7 +223,7 @@ class QuantizedKVCache:
             q, q_at, qsn, qsh, qn, qh = self._rows(q, "q")
             if qn != n or q.dtype != dtype:
                 raise ValueError("q and k must have the same tokens and dtype")
-            out = torch.empty((n, qh, self.head_dim), dtype=dtype, device=self.device)
+            out = q.new_empty((n, qh, self.head_dim))
             a.q, a.q_stride_n, a.q_stride_h, a.n_q_heads, a.out = q_at, qsn, qsh, qh, out.data_ptr()
         keep = []
         for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
@@ -294,7 +294,7 @@ class QuantizedKVCache:
         if h == 0 or h % self.n_kv_heads != 0:
             raise ValueError("%d query heads do not divide over %d kv heads" % (h, self.n_kv_heads))
         if out is None:
-            out = torch.empty((n, h, self.head_dim), dtype=q.dtype, device=self.device)
+            out = q.new_empty((n, h, self.head_dim))
         else:
             self._on_device(out, "out")
             if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() & 15:
@@ -326,7 +326,7 @@ class QuantizedKVCache:
         at = ctypes.byref(a)
         need = L.gl_kv_attend_workspace_bytes(at)
         if need:
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+            ws = self.k_codes.new_empty(need)
             a.workspace, a.workspace_bytes = ws.data_ptr(), need
         status = L.gl_kv_attend(at, _lib.current_stream_ptr(self.device))
         if status:

@@ -310,6 +310,30 @@ def test_attend_queries_of_any_size(lib, magnitude):
     _check_attend(cache, table, [198], [2], q, None, cache.attend(q, KVBatch(table, _i32([198])), scale=0.1 / magnitude), scale=0.1 / magnitude)
 
 
+@pytest.mark.parametrize("scale", [-0.1, 0.0])
+@pytest.mark.parametrize("kernel", [1, 2])
+def test_attend_with_a_scale_of_zero_or_below(lib, scale, kernel):
+    from gemlite_b200 import KVBatch
+    cache, table = make_cache([300, 40], 2, 64, "fp8", 32, seed=15)
+    q = _randn(6, 6, 8, 64)
+    _check_attend(cache, table, [297, 37], [3, 3], q, None, cache.attend(q, KVBatch(table, _i32([297, 37])), scale=scale, kernel_override=kernel),
+                  scale=scale, rounds_codes=kernel == 2)
+
+
+def test_attend_scales_far_apart_for_many_rows(lib):
+    """The kernel for many rows folds scales into the codes only where they are near each other."""
+    from gemlite_b200 import KVBatch
+    for fmt in FMTS:
+        cache, table = make_cache([520], 1, 128, fmt, 16, seed=18)
+        page = int(table[0, 3])
+        cache.v_scales[page, :, 5] *= 2.0 ** 20
+        cache.k_scales[int(table[0, 7])] *= 2.0 ** -13
+        cache.v_scales[int(table[0, 20])] *= 2.0 ** -30
+        cache.v_scales[int(table[0, 21])] = 0.0
+        q = _randn(3, 20, 8, 128, scale=2.0)
+        _check_attend(cache, table, [500], [20], q, None, cache.attend(q, KVBatch(table, _i32([500])), scale=0.05), scale=0.05)
+
+
 def test_attend_strided_and_misaligned_queries(lib):
     from gemlite_b200 import KVBatch
     cache, table = make_cache([100], 2, 64, "fp8", 16, seed=10)
