@@ -10,6 +10,10 @@
 // numbers).  q is fp16 already or is brought there from bf16 by a power of two per row (its largest channel lands in
 // [1, 2): channels 2^-14 of it and smaller lose bits, at most 2^-25 of the largest each).  P carries a factor 2^15, which
 // leaves the fp16 format 39 binary orders below the largest weight before a weight is lost.
+//
+// Bound by the cache's bytes, then by issue slots (conversion, about 500 instructions per 32 tokens of 128 channels).  32 decoding
+// sequences of 500 to 16000 tokens, 64 / 8 heads of 128 in fp8 (559 MB): 100 us, 5.6 TB/s.  One sequence of 131000 tokens, 8 / 1 heads,
+// int8 (35 MB): 20 us, of which the tokens take 5.
 #include "gl_kv_attend.cuh"
 #include <mutex>
 
