@@ -208,7 +208,7 @@ class QuantizedKVCache:
 
         Arithmetic is fp32 and rounded once.  A row (one token's head) with an infinity or NaN is stored as codes 0 with the
         scale NaN.  A position outside the table gives NaN queries and such a key row.  Tokens whose page does not exist are
-        dropped.  A page must not be written for two sequences in one call.  Rows of the result that belong to no
+        dropped.  A page must not be written for two sequences, or twice for one, in a call.  Rows of the result that belong to no
         sequence are not written."""
         k, k_at, ksn, ksh, n, _ = self._rows(k, "k", self.n_kv_heads)
         v, v_at, vsn, vsh, vn, _ = self._rows(v, "v", self.n_kv_heads)

@@ -462,6 +462,51 @@ def test_graph_capture_streams_and_repeats(lib):
     assert torch.equal(outs[0], later) and torch.equal(outs[1], later) and not torch.equal(later, want)
 
 
+@pytest.mark.parametrize("T,hq", [(5, 4), (24, 8)])
+def test_masks_of_other_widths_and_strides(lib, T, hq):
+    """Narrower than the new tokens (the rest counts as False), no columns at all, one row for all (stride 0), values other than 1."""
+    from gemlite_b200 import KVBatch
+    cache, table = make_cache([50 + T], 2, 64, "int8", 16, seed=16)
+    q, batch = _randn(7, T, hq, 64), KVBatch(table, _i32([50]))
+    narrow = torch.ones(T, 3, dtype=torch.bool, device=DEV)
+    for mask in (narrow, narrow[:, :0], narrow[:1].expand(T, 3), torch.nn.functional.pad(narrow, (0, 40))[:, :T + 30]):
+        want = torch.zeros(T, T, dtype=torch.bool, device=DEV)
+        w = min(mask.shape[1], T)
+        want[:, :w] = mask[:, :w]
+        _check_attend(cache, table, [50], [T], q, want, cache.attend(q, batch, mask=mask))
+    wide = torch.randint(0, 256, (T, T), dtype=torch.uint8, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+    wide[0] = 0
+    _check_attend(cache, table, [50], [T], q, wide != 0, cache.attend(q, batch, mask=wide))
+
+
+def test_whole_step_in_a_graph(lib):
+    """Write, attend and read captured once, replayed with new lengths and inputs in place."""
+    from gemlite_b200 import KVBatch, rotary_table
+    cache, table = make_cache([200, 200], 2, 64, "int4", 16, seed=17)
+    other, _ = make_cache([200, 200], 2, 64, "int4", 16, seed=17)
+    cs, ctx, pos = rotary_table(256, 64, device=DEV), _i32([10, 40]), _i32([10, 40])
+    q, k, v = _randn(1, 2, 8, 64), _randn(2, 2, 2, 64), _randn(3, 2, 2, 64)
+
+    def step(c):
+        b = KVBatch(table, ctx, max_len=200)
+        y = c.attend(c.write(q, k, v, b, positions=pos, cos_sin=cs), b)
+        return (y, *c.read(table, ctx + 1, max_len=200, out_dtype=torch.float16))
+
+    step(cache), step(other)                     # (the caches hold the same; the first step writes to both)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        got = step(cache)
+    for n in range(3):
+        q.copy_(_randn(10 + n, 2, 8, 64)), k.copy_(_randn(20 + n, 2, 2, 64)), v.copy_(_randn(30 + n, 2, 2, 64))
+        ctx.add_(_i32([1, 50])), pos.copy_(ctx)
+        g.replay()
+        want = step(other)
+        torch.cuda.synchronize()
+        assert bool(got[0].isfinite().all()) and all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 # ---- refusals ----------------------------------------------------------------------------------------------------------------
 def test_refusals(lib):
     from gemlite_b200 import KVBatch, QuantizedKVCache
