@@ -21,7 +21,6 @@ allocator per call, so calls on several streams and captured graphs do not share
 """
 import ctypes
 import math
-import struct
 from typing import Optional
 
 import torch
@@ -34,7 +33,6 @@ KV_FORMATS = {"fp8": 0, "int8": 1, "int4": 2}
 _DTYPE_CODES = {torch.float16: DType.FP16.value, torch.bfloat16: DType.BF16.value, torch.float32: DType.FP32.value}
 _HALF_CODES = {torch.float16: DType.FP16.value, torch.bfloat16: DType.BF16.value}
 _INT32_MAX = 2 ** 31 - 1
-_POINTERS = struct.Struct("=9Q")       # the argument struct begins with the addresses of the cache's and the batch's tensors
 
 
 def rotary_table(max_positions: int, rot_dim: int, base: float = 10000.0, device="cuda:0") -> Tensor:
@@ -67,26 +65,17 @@ class KVBatch:
 
     def __init__(self, page_table: Tensor, ctx_lens: Tensor, q_offsets: Optional[Tensor] = None,
                  max_len: Optional[int] = None, max_new: Optional[int] = None):
-        d = self.__dict__
-        d["page_table"], d["ctx_lens"], d["q_offsets"] = page_table, ctx_lens, q_offsets
-        d["max_len"], d["max_new"] = max_len and self._bound(max_len), max_new and self._bound(max_new)
+        self.page_table, self.ctx_lens, self.q_offsets = page_table, ctx_lens, q_offsets
+        self.max_len = None if max_len is None else max(0, min(int(max_len), _INT32_MAX))
+        self.max_new = None if max_new is None else max(0, min(int(max_new), _INT32_MAX))
         self._check()
-
-    @staticmethod
-    def _bound(n):
-        return None if n is None else max(0, min(int(n), _INT32_MAX))
-
-    def __setattr__(self, name, value):
-        """Tensors and bounds may be replaced; the next call checks them together."""
-        self.__dict__[name] = self._bound(value) if name in ("max_len", "max_new") else value
-        self.__dict__["_checked"] = False
 
     def __reduce__(self):
         return type(self), (self.page_table, self.ctx_lens, self.q_offsets, self.max_len, self.max_new)
 
     def _check(self):
-        d = self.__dict__
-        page_table, ctx_lens, q_offsets = _index_tensor(d["page_table"], "page_table", 2), _index_tensor(d["ctx_lens"], "ctx_lens", 1), d["q_offsets"]
+        """Tensors may be replaced: the next call comes here again."""
+        page_table, ctx_lens, q_offsets = _index_tensor(self.page_table, "page_table", 2), _index_tensor(self.ctx_lens, "ctx_lens", 1), self.q_offsets
         shape, device = tuple(page_table.shape), page_table.device
         if ctx_lens.shape[0] != shape[0]:
             raise ValueError("ctx_lens has %d entries for %d sequences" % (ctx_lens.shape[0], shape[0]))
@@ -94,9 +83,8 @@ class KVBatch:
             raise ValueError("q_offsets must have %d entries (sequences + 1), got %d" % (shape[0] + 1, q_offsets.shape[0]))
         if ctx_lens.device != device or (q_offsets is not None and q_offsets.device != device):
             raise ValueError("page_table, ctx_lens and q_offsets must be on one device")
-        d["shape"], d["device"], d["table_stride"] = shape, device, page_table.stride(0)
-        d["_at"] = page_table.data_ptr, ctx_lens.data_ptr, int if q_offsets is None else q_offsets.data_ptr
-        d["_checked"] = True
+        self.device, self.shape, self.table_stride = device, shape, page_table.stride(0)
+        self._checked = page_table, ctx_lens, q_offsets
 
 
 class QuantizedKVCache:
@@ -129,14 +117,16 @@ class QuantizedKVCache:
 
     def __setattr__(self, name, value):
         if name != "_args":
-            self.__dict__["_args"] = None
-        self.__dict__[name] = value
+            object.__setattr__(self, "_args", None)
+        object.__setattr__(self, name, value)
 
     def __reduce__(self):
         return type(self).from_buffers, (self.k_codes, self.v_codes, self.k_scales, self.v_scales, self.kv_format, self.k_zeros, self.v_zeros)
 
-    def _recheck(self):
-        self._take(self.k_codes, self.v_codes, self.k_scales, self.v_scales, self.kv_format, self.k_zeros, self.v_zeros)
+    def _check(self):
+        """The buffers are those, and lie where, the last check saw them; else they are checked again."""
+        if self._args is None or self._addresses != [at() for at in self._address_of]:
+            self._take(self.k_codes, self.v_codes, self.k_scales, self.v_scales, self.kv_format, self.k_zeros, self.v_zeros)
 
     def _take(self, k_codes, v_codes, k_scales, v_scales, kv_format, k_zeros, v_zeros):
         if kv_format not in KV_FORMATS:
@@ -163,11 +153,13 @@ class QuantizedKVCache:
         self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
         self.k_zeros, self.v_zeros = k_zeros, v_zeros
         a = _lib.GLKvArgs()
+        for name in ("k_codes", "v_codes", "k_scales", "v_scales", "k_zeros", "v_zeros"):
+            setattr(a, name, _lib.ptr(getattr(self, name)))
         a.format, a.num_pages, a.page_size = KV_FORMATS[kv_format], self.num_pages, self.page_size
         a.n_kv_heads, a.head_dim = self.n_kv_heads, self.head_dim
-        # addresses are taken anew by every call
-        self._at = (k_codes.data_ptr, v_codes.data_ptr, k_scales.data_ptr, v_scales.data_ptr, k_zeros.data_ptr if int4 else int, v_zeros.data_ptr if int4 else int)
-        self._args = bytes(a)[_POINTERS.size:]
+        self._address_of = tuple(t.data_ptr for t in (k_codes, v_codes, k_scales, v_scales, k_zeros, v_zeros) if t is not None)
+        self._addresses = [at() for at in self._address_of]
+        self._args = bytes(a)
 
     # -- argument plumbing (a decode step makes these calls once per layer: what they cost the host counts) ----------------------
     def _on_device(self, t, what):
@@ -198,15 +190,17 @@ class QuantizedKVCache:
         return x, at, sn, sh, n, h
 
     def _batch_args(self, batch, n):
-        if not batch._checked:
+        page_table, ctx_lens, q_offsets = batch._checked
+        if batch.page_table is not page_table or batch.ctx_lens is not ctx_lens or batch.q_offsets is not q_offsets:
             batch._check()
-        (kc, vc, ks, vs, kz, vz), (pt, lens, off) = self._at, batch._at
-        a = _lib.GLKvArgs.from_buffer_copy(_POINTERS.pack(kc(), vc(), ks(), vs(), kz(), vz(), pt(), lens(), off()) + self._args)
+            page_table, ctx_lens, q_offsets = batch._checked
         if batch.device != self.device:
             raise ValueError("the batch is on %s, the cache on %s" % (batch.device, self.device))
+        a = _lib.GLKvArgs.from_buffer_copy(self._args)
         B, P = batch.shape
-        a.page_table_stride = batch.table_stride
-        if batch.q_offsets is not None:
+        a.page_table, a.page_table_stride, a.lens = page_table.data_ptr(), batch.table_stride, ctx_lens.data_ptr()
+        if q_offsets is not None:
+            a.q_offsets = q_offsets.data_ptr()
             a.max_new = n if batch.max_new is None else batch.max_new
         elif B > 0:
             if n % B != 0:
@@ -242,8 +236,7 @@ class QuantizedKVCache:
         scale NaN.  A position outside the table gives NaN queries and such a key row.  Tokens whose page does not exist are
         dropped.  A page must not be written for two sequences, or twice for one, in a call.  Rows of the result that belong to no
         sequence are not written."""
-        if self._args is None:
-            self._recheck()
+        self._check()
         k, k_at, ksn, ksh, n, _ = self._rows(k, "k", self.n_kv_heads)
         v, v_at, vsn, vsh, vn, _ = self._rows(v, "v", self.n_kv_heads)
         dtype = k.dtype
@@ -300,8 +293,7 @@ class QuantizedKVCache:
         and where a page does not exist.  max_len defaults to what the table holds; longer sequences are cut there."""
         if out_dtype not in _DTYPE_CODES:
             raise NotImplementedError("out_dtype %s is not supported" % out_dtype)
-        if self._args is None:
-            self._recheck()
+        self._check()
         batch = KVBatch(page_table, lens)
         a = self._batch_args(batch, 0)
         if max_len is not None:
@@ -326,8 +318,7 @@ class QuantizedKVCache:
         new tokens up to the query's own (single tokens, prompt chunks).  A row that sees nothing gives zeros; what a row does not
         see has no influence on it, whatever those slots hold.  scale defaults to 1 / sqrt(head_dim).
         Result like q (contiguous); rows that belong to no sequence are not written."""
-        if self._args is None:
-            self._recheck()
+        self._check()
         q, at, sn, sh, n, h = self._rows(q, "q")
         if h == 0 or h % self.n_kv_heads != 0:
             raise ValueError("%d query heads do not divide over %d kv heads" % (h, self.n_kv_heads))

@@ -104,10 +104,9 @@ def test_replaced_batch_tensors_are_checked_and_used(lib, caught):
     batch.q_offsets = torch.zeros(3, dtype=torch.int32)
     with pytest.raises(ValueError, match="q_offsets"):
         _write(cache, batch)
-    batch.q_offsets = torch.zeros(2, dtype=torch.int32)
-    batch.max_len, batch.max_new = 2 ** 40, -1
+    batch.q_offsets, batch.max_new = torch.zeros(2, dtype=torch.int32), 7
     _write(cache, batch)
-    assert (caught[-1].max_len, caught[-1].max_new) == (2 ** 31 - 1, 0)
+    assert (caught[-1].q_offsets, caught[-1].max_new) == (batch.q_offsets.data_ptr(), 7)
 
 
 def test_copies_of_a_batch(lib, caught):
