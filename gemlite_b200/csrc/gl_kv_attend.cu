@@ -20,7 +20,6 @@
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kTinyScale = 1e-30f;
 constexpr int kTile = 32;          // tokens that a warp takes at a time
 constexpr int kWarps = 4;
 constexpr int kStages = 3;

@@ -28,6 +28,11 @@ constexpr int kKvTcRows = 256;
 int kv_allow_smem(const void* kernel, int bytes);
 int gl_kv_attend_tc_launch(const KvAttendParams& p, int head_dim, int format, int x_dtype, cudaStream_t st);
 
+// Values whose scale is smaller count as zero: their codes become zeros under this scale.  Their term of the denominator is at most
+// 2^15 / kTinyScale, 2^95, so that the 2^30 tokens that a table may hold stay below 2^126.  (With 1e-30, 2^115, a
+// dozen thousand slots that were never written made it infinite, and the row zero.)
+constexpr float kTinyScale = 1e-24f;
+
 template <typename T> struct IsHalf { static constexpr bool value = false; };
 template <> struct IsHalf<__half> { static constexpr bool value = true; };
 

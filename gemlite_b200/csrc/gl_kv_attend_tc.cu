@@ -252,7 +252,7 @@ __device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh
     const uint32_t hi = __reduce_max_sync(0xffffffffu, plain ? bits : 0u), lo = __reduce_min_sync(0xffffffffu, plain ? bits : 0x7f7fffffu);
     const bool apart = (draft && p.mask != nullptr) || (int)(hi >> 23) - (int)(lo >> 23) >= (values ? kSpreadV<FMT> : kSpread);
     const int e = apart ? 0 : pow2_above(hi) - (values ? 0 : kRoom<FMT>);
-    const bool number = fabsf(scale) < INFINITY, none = apart && scale < 1e-30f;
+    const bool number = fabsf(scale) < INFINITY, none = apart && scale < kTinyScale;
     const uint32_t valid = __ballot_sync(0xffffffffu, rows.slot != kNoSlot);
     // Values that are not numbers would reach every row through P V', so V' is 0 there, and the exponent is NaN, which only the
     // rows that see the token meet.  (e4m3's NaN codes matter where some rows do not see the token.)
@@ -299,7 +299,7 @@ __device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh
       }
     }
     if (values) {
-      const float v = none ? 1e-30f : scale;
+      const float v = none ? kTinyScale : scale;
       m.col_lv[w * 32 + lane] = (bad >> lane) & 1u ? __int_as_float(0x7fc00000) : apart ? __log2f(v) : (float)e;
       m.col_rv[w * 32 + lane] = apart ? __frcp_rn(v) : pow2(-e);
     } else {

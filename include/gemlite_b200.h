@@ -302,8 +302,8 @@ GL_API int gl_silu_mul(const void* gate_up, void* out, int32_t M, int32_t inter,
  *
  * Cache layout (all contiguous): codes [num_pages, n_kv_heads, page_size, row], row = head_dim bytes (GL_KV_FP8 e4m3,
  * GL_KV_INT8) or head_dim / 2 bytes (GL_KV_INT4, even channel in the low nibble); scales fp32 [num_pages, n_kv_heads,
- * page_size], positive; GL_KV_INT4: zeros uint8 of the same shape, 0..15.  value = (code - zero) * scale.  Codes are
- * 16-byte aligned; head_dim is 64 or 128.
+ * page_size], positive or 0; GL_KV_INT4: zeros uint8 of the same shape, 0..15.  value = (code - zero) * scale; attention takes
+ * values of a scale below 1e-24 for zeros.  Codes are 16-byte aligned; head_dim is 64 or 128.
  *
  * Batch: sequence b holds lens[b] tokens already (gl_kv_read: the tokens to read); its new tokens are rows
  * q_offsets[b] .. q_offsets[b+1] of the token-major operands (q_offsets NULL: n_tokens / batch rows each), its token p
