@@ -7,8 +7,9 @@
 //   S = q K'^T,  P = 2^(a S + log2 VS - M + 7),  O += P V',  l += sum P / VS,  a = log2(e) c KS (times q's power of two)
 // and a score costs one multiply-add, one exponential, one maximum and one addition.  None of these numbers is a subnormal
 // fp16 number as long as the scales lie near each other (kSpread, kSpreadV), so the choice of KS and VS changes no bit.  Where
-// they lie further apart, and where tiles hold new tokens under a mask (a token that a row does not see must not round what it
-// sees), K' or V' stay the codes, and ks[p], or log2 vs[p] and 1 / vs[p], go to the scores, as in the other kernel.
+// they lie further apart, and in tiles that some row of the unit does not see all of (new tokens under a mask; without one those
+// behind the first row's own: a token that a row does not see must not round what it sees), K' or V' stay the codes, and ks[p],
+// or log2 vs[p] and 1 / vs[p], go to the scores, as in the other kernel.
 // M is a maximum of the exponents that lags: it is raised, and O and l are scaled, only when a row's new maximum is more than
 // 2^8 above it (P stays below 2^15 then, fp16's range, and keeps 31 binary orders below M).
 //
@@ -193,7 +194,7 @@ __device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh
   bool have = walk.next(p, blockIdx.x, pc);
   int tile = have ? pc.t0 : 0;
   // A tile two ahead: its page numbers are on their way while the codes of the one before are fetched.
-  struct Item { int page, place, head; uint32_t flags; };                 // flags: 1 tile exists, 2 token within the sequence, 4 new tokens
+  struct Item { int page, place, head; uint32_t flags; };                 // flags: 1 tile exists, 2 token within the sequence, 4 not all rows see all of it
   auto fetch = [&]() {
     Item it{-1, 0, 0, 0u};
     while (have && tile >= pc.t1) {
@@ -203,7 +204,8 @@ __device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh
     if (have) {
       const int pos = tile * kKvTile + w * 32 + lane;
       it.head = pc.head;
-      it.flags = 1u | ((tile + 1) * kKvTile > pc.s.ctx ? 4u : 0u);
+      const int seen = pc.s.ctx + (p.mask == nullptr ? pc.row0 / p.group + 1 : 0);      // by every row of the unit
+      it.flags = 1u | ((tile + 1) * kKvTile > seen ? 4u : 0u);
       if (pos < pc.s.len) {
         const int pi = p.page_shift >= 0 ? pos >> p.page_shift : pos / kb.page_size;
         it.place = pos - pi * kb.page_size;
@@ -245,12 +247,12 @@ __device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh
 #pragma unroll 1
   for (int n = 0; flags & 1u; ++n) {
     const int st = n & 1;
-    const bool draft = flags & 4u;
+    const bool parted = flags & 4u;
     // the power of two, and whether the scales are near enough to each other
     const uint32_t bits = __float_as_uint(scale);
     const bool plain = bits - 1u < 0x7f7fffffu;                          // positive and finite
     const uint32_t hi = __reduce_max_sync(0xffffffffu, plain ? bits : 0u), lo = __reduce_min_sync(0xffffffffu, plain ? bits : 0x7f7fffffu);
-    const bool apart = (draft && p.mask != nullptr) || (int)(hi >> 23) - (int)(lo >> 23) >= (values ? kSpreadV<FMT> : kSpread);
+    const bool apart = parted || (int)(hi >> 23) - (int)(lo >> 23) >= (values ? kSpreadV<FMT> : kSpread);
     const int e = apart ? 0 : pow2_above(hi) - (values ? 0 : kRoom<FMT>);
     const bool number = fabsf(scale) < INFINITY, none = apart && scale < kTinyScale;
     const uint32_t valid = __ballot_sync(0xffffffffu, rows.slot != kNoSlot);
@@ -274,7 +276,7 @@ __device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh
 #pragma unroll
       for (int i = 0; i < G; ++i) {
         const int t = c_tok + (g + i) * C::TPI;
-        if (FMT == GL_KV_FP8 && values && draft) {
+        if (FMT == GL_KV_FP8 && values && parted) {
           const uint32_t m = 0x7f7f7f7fu, one = 0x01010101u;
           const bool nan = (((((u[i].x & m) + one) | ((u[i].y & m) + one) | ((u[i].z & m) + one) | ((u[i].w & m) + one)) & 0x80808080u) != 0);
           const uint32_t who = __reduce_or_sync(0xffffffffu, nan ? 1u << t : 0u);

@@ -26,3 +26,30 @@ def test_long_stretches_of_zero_scales(lib, fmt, kernel):
     q = _randn(33, B, hkv, 64)
     out = cache.attend(q, KVBatch(table, _i32([n - 1] * B), max_len=n, max_new=1), kernel_override=kernel)
     _check_attend(cache, table, [n - 1] * B, [1] * B, q, None, out, rounds_codes=kernel == 2)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("ctx,hq", [(0, 16), (61, 16), (700, 16), (700, 64), (61, 2)])
+def test_later_tokens_of_a_chunk_do_not_reach_earlier_rows(lib, fmt, ctx, hq):
+    """No mask: row i sees the new tokens up to its own.  Whatever scales and codes the last one holds, the rows before it keep
+    every bit."""
+    from gemlite_b200 import KVBatch
+    T, hkv = 40, 2
+    cache, table = make_cache([ctx + T], hkv, 128, fmt, 16, seed=30)
+    q = _randn(31, T, hq, 128, dtype=torch.float16, scale=1.5)
+    batch = KVBatch(table, _i32([ctx]), max_len=ctx + T, max_new=T)
+    page, at = int(table[0, (ctx + T - 1) // 16]), (ctx + T - 1) % 16
+    for kernel in (0, 1, 2):
+        want = cache.attend(q, batch, kernel_override=kernel)
+        kept = [t.clone() for t in (cache.k_scales, cache.v_scales, cache.k_codes, cache.v_codes)]
+        for ks, vs, code in ((2.0 ** -14, 1.0, None), (1.0, 2.0 ** -14, None), (1.0, 2.0 ** 6, None), (2.0 ** 20, 2.0 ** 20, 0x55), (0.0, 0.0, 0),
+                             (math.inf, math.inf, 0x7F), (math.nan, math.nan, 0xFF), (1.0, 1.0, 0x7F)):
+            cache.k_scales[page, :, at] *= ks
+            cache.v_scales[page, :, at] *= vs
+            if code is not None:
+                cache.k_codes[page, :, at] = code
+                cache.v_codes[page, :, at] = code
+            got = cache.attend(q, batch, kernel_override=kernel)
+            for t, old in zip((cache.k_scales, cache.v_scales, cache.k_codes, cache.v_codes), kept):
+                t.copy_(old)
+            assert torch.equal(got[:-1], want[:-1]), (kernel, ks, vs, code)
