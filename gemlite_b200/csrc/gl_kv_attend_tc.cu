@@ -11,7 +11,8 @@
 // behind the first row's own: a token that a row does not see must not round what it sees), K' or V' stay the codes, and ks[p],
 // or log2 vs[p] and 1 / vs[p], go to the scores, as in the other kernel.
 // M is a maximum of the exponents that lags: it is raised, and O and l are scaled, only when a row's new maximum is more than
-// 2^8 above it (P stays below 2^15 then, fp16's range, and keeps 31 binary orders below M).
+// 2^8 above it (P stays below 2^15 then, fp16's range, and keeps 31 binary orders below M).  Each row decides for itself: what its
+// neighbours see does not reach its roundings.
 //
 // One persistent block per SM, 17 working warps:
 //   warps 0-3, 4-7    two streams of 128 rows: scores out of TMEM, weights back into TMEM (over the scores), rescaling, output
@@ -510,7 +511,7 @@ __device__ __forceinline__ void stream_role(const KvAttendParams& p, Shared& sh,
         }
         const bool raise = t_top > m_used + kRaise || (m_used == -INFINITY && t_top != -INFINITY);
         if (__any_sync(0xffffffffu, raise)) {
-          const float m_new = fmaxf(m_used, t_top), f = m_used == m_new ? 1.f : kv_exp2(m_used - m_new);
+          const float m_new = raise ? t_top : m_used, f = raise ? kv_exp2(m_used - m_new) : 1.f;
           l *= f;
           m_used = m_new;
           if (i > 0) {                                                // (s_full: the products before this tile's scores are done)

@@ -53,3 +53,27 @@ def test_later_tokens_of_a_chunk_do_not_reach_earlier_rows(lib, fmt, ctx, hq):
             for t, old in zip((cache.k_scales, cache.v_scales, cache.k_codes, cache.v_codes), kept):
                 t.copy_(old)
             assert torch.equal(got[:-1], want[:-1]), (kernel, ks, vs, code)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("B,ctx,T", [(1, 61, 40), (1, 700, 40), (24, 700, 40), (48, 1100, 16)])
+def test_unseen_tokens_over_many_tiles(lib, fmt, B, ctx, T):
+    """One draft token that only row 1 sees gets a key 64 times as large, so that row 1's maximum rises far on the last tile: all
+    other rows keep every bit.  24 and 48 sequences: pieces of many tiles, whose running maxima matter."""
+    from gemlite_b200 import KVBatch
+    hkv, hq = 8, 64
+    cache, table = make_cache([ctx + T] * B, hkv, 128, fmt, 16, seed=30)
+    q = _randn(31, B * T, hq, 128, dtype=torch.float16, scale=1.5)
+    mask = torch.ones(T, T, dtype=torch.bool, device=DEV).tril()
+    mask[:, 1] = False
+    mask[1, 1] = True
+    mask = mask.repeat(B, 1)
+    batch = KVBatch(table, _i32([ctx] * B), max_len=ctx + T, max_new=T)
+    want = cache.attend(q, batch, mask=mask)
+    others = torch.arange(B * T, device=DEV) % T != 1
+    pages = table[:, (ctx + 1) // 16].long()
+    for factor in (64.0, 2.0 ** -20):
+        cache.k_scales[pages, :, (ctx + 1) % 16] *= factor
+        got = cache.attend(q, batch, mask=mask)
+        assert not torch.equal(got[~others], want[~others])
+        assert torch.equal(got[others], want[others])
