@@ -262,7 +262,8 @@ __global__ void __launch_bounds__(256, 3) kv_write_kernel(const WriteParams p) {
           lo = fminf(lo, __shfl_xor_sync(gmask, lo, o));
           hi = fmaxf(hi, __shfl_xor_sync(gmask, hi, o));
         }
-        const float scale = fmaxf(__fdiv_rn(__fsub_rn(hi, lo), 15.f), 1e-6f);
+        const float span = __fsub_rn(hi, lo);                      // (of bf16 numbers beyond 2^127 it is no fp32 number)
+        const float scale = fmaxf(span < INFINITY ? __fdiv_rn(span, 15.f) : __fsub_rn(__fdiv_rn(hi, 15.f), __fdiv_rn(lo, 15.f)), 1e-6f);
         const float zero = fminf(fmaxf(rintf(__fdiv_rn(-lo, scale)), 0.f), 15.f);
         uint32_t o = 0;
 #pragma unroll

@@ -77,3 +77,21 @@ def test_unseen_tokens_over_many_tiles(lib, fmt, B, ctx, T):
         got = cache.attend(q, batch, mask=mask)
         assert not torch.equal(got[~others], want[~others])
         assert torch.equal(got[others], want[others])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_rows_that_span_more_than_fp32(lib, fmt):
+    """Finite bf16 rows keep finite values, also where the largest less the smallest number is beyond fp32: each comes back within
+    half a step (e4m3: 2^-4 of it, codes below its smallest normal number 2^-10 of the scale).  2.7e38 and -3e38 over 15
+    steps are 3.8e37 each: 8 below the zero point (-3.04e38) and 7 above it (2.66e38) are fp32 numbers."""
+    from gemlite_b200 import KVBatch
+    cache, table = make_cache([8], 1, 64, fmt, 16, seed=1)
+    x = _randn(1, 2, 1, 64)
+    x[0, 0, 0], x[0, 0, 1], x[0, 0, 2] = 2.7e38, -3e38, 1e38
+    batch = KVBatch(table, _i32([0]))
+    cache.write(None, x, x, batch)
+    for got in cache.read(table, _i32([2]), max_len=2, out_dtype=torch.float32):
+        scale = cache.k_scales[int(table[0, 0]), 0, :2, None].double()
+        step = torch.maximum(2.0 ** -4 * x[:, 0].double().abs(), 2.0 ** -10 * scale) if fmt == "fp8" else 0.5 * scale
+        top = x[:, 0].double().abs().amax(-1, keepdim=True)
+        assert bool(((got[0, :, 0].double() - x[:, 0].double()).abs() <= step + 2.0 ** -20 * top).all())
