@@ -123,7 +123,9 @@ __device__ __forceinline__ void normalise(float (&x)[R][8], const float (&w)[8],
   }
   for (; o > 0; o >>= 1) mine += __shfl_xor_sync(gmask, mine, o);
   const float mean = (float)(mine * (1.0 / (LPR * 8)));
-  const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(mean, eps)));
+  float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(mean, eps)));
+  // bf16 numbers beyond 2^64: their mean square, at most 2^256, goes through fp32 with 2^-128 (eps is nothing beside it)
+  if (mean == INFINITY) inv = __fmul_rn(__fdiv_rn(1.0f, __fsqrt_rn((float)(mine * (0x1p-128 / (LPR * 8))))), 0x1p-64f);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const float f = R == 1 ? inv : __shfl_sync(gmask, inv, ((threadIdx.x & 31) / LPR) * LPR + (r >> 1) * (LPR / 2) + (r & 1) * (LPR / 4));

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from tests.kv_util import make_cache
+from tests.kv_util import make_cache, norm64
 from tests.test_gpu_kv_cache import DEV, FMTS, _check_attend, _i32, _randn
 
 pytestmark = pytest.mark.gpu
@@ -95,3 +95,23 @@ def test_rows_that_span_more_than_fp32(lib, fmt):
         step = torch.maximum(2.0 ** -4 * x[:, 0].double().abs(), 2.0 ** -10 * scale) if fmt == "fp8" else 0.5 * scale
         top = x[:, 0].double().abs().amax(-1, keepdim=True)
         assert bool(((got[0, :, 0].double() - x[:, 0].double()).abs() <= step + 2.0 ** -20 * top).all())
+
+
+@pytest.mark.parametrize("size", [1e18, 1e19, 1e25, 3e38])
+def test_norm_of_large_heads(lib, size):
+    """Head norms of bf16 rows whose mean square is no fp32 number; a row with an infinity among them stays no number."""
+    from gemlite_b200 import KVBatch
+    cache, table = make_cache([8], 1, 64, "int8", 16, seed=1)
+    x = _randn(1, 3, 6, 64)
+    x = (x / x.abs().amax().float() * size).to(torch.bfloat16)
+    x[2, :, 7] = math.inf
+    w = 1 + 0.3 * _randn(2, 64, dtype=torch.float32)
+    k = x[:, :1]
+    out = cache.write(x, k, k, KVBatch(table, _i32([0])), q_norm=w, k_norm=w)
+    want = norm64(x.double(), w, 1e-6)[:2]
+    # one rounding to bf16; the reciprocal root is rounded to 2^-149 beside 2^-128 at the least
+    assert bool(((out[:2].double() - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -22 + 8 * 2.0 ** -24) * want.abs()).all())
+    assert bool(out[2, :, 7].isnan().all())
+    key = cache.read(table, _i32([3]), max_len=3, out_dtype=torch.float32)[0]
+    scale = want[:, :1].abs().amax(-1, keepdim=True) / 127
+    assert bool(((key[0, :2].double() - want[:, :1]).abs() <= 0.5 * scale * (1 + 2.0 ** -10)).all()) and bool(key[0, 2].isnan().all())
