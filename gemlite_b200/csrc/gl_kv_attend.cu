@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kWarps * 32, kv_mma_blocks(D, FMT, NR)) kv_att
       if (i < mine && pos < c1) {
         const int pi = p.page_shift >= 0 ? pos >> p.page_shift : pos / kb.page_size;
         place_next = pos - pi * kb.page_size;
-        page_next = __ldg(kb.page_table + pt_row + pi);
+        page_next = kv_load(kb.page_table + pt_row + pi);
       }
     };
     look_up(0);

@@ -37,6 +37,11 @@ template <typename T> struct IsHalf { static constexpr bool value = false; };
 template <> struct IsHalf<__half> { static constexpr bool value = true; };
 
 #ifdef __CUDACC__
+// Page numbers, codes and scales: from L2.  Not by the read-only path (ld.global.nc), which is for memory that nobody writes
+// during a kernel: this launch may begin while the write that it waits for still runs.  (Codes by L1: a chunk of 1000 tokens over 7000
+// 408 us, past it 402.)
+template <typename V> __device__ __forceinline__ V kv_load(const V* p) { return __ldcg(p); }
+
 // row of a token's (page, head, place) in the cache as a 32-bit number (gl_kv_check: there are fewer than 2^32 - 1)
 constexpr uint32_t kNoSlot = 0xffffffffu;
 __device__ __forceinline__ uint32_t kv_slot32(const KvBatch& kb, int page, int head, int place) {

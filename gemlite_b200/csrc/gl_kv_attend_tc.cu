@@ -210,7 +210,7 @@ __device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh
       if (pos < pc.s.len) {
         const int pi = p.page_shift >= 0 ? pos >> p.page_shift : pos / kb.page_size;
         it.place = pos - pi * kb.page_size;
-        it.page = __ldg(kb.page_table + (int64_t)walk.b * kb.pt_stride + pi);
+        it.page = kv_load(kb.page_table + (int64_t)walk.b * kb.pt_stride + pi);
         it.flags |= 2u;
       }
       ++tile;
@@ -229,9 +229,9 @@ __device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh
     return r;
   };
   auto take = [&](const Rows& r, int piece) {
-    if (r.in_line) return __ldg(reinterpret_cast<const uint4*>(r.at + piece * (C::TPI * C::RB)));
+    if (r.in_line) return kv_load(reinterpret_cast<const uint4*>(r.at + piece * (C::TPI * C::RB)));
     const uint32_t s = __shfl_sync(0xffffffffu, r.slot, c_tok + piece * C::TPI);
-    return s != kNoSlot ? __ldg(reinterpret_cast<const uint4*>(codes + (int64_t)s * C::RB)) : make_uint4(0, 0, 0, 0);
+    return s != kNoSlot ? kv_load(reinterpret_cast<const uint4*>(codes + (int64_t)s * C::RB)) : make_uint4(0, 0, 0, 0);
   };
 
   Item nxt = fetch();
@@ -242,8 +242,8 @@ __device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh
   uint4 u[G];
 #pragma unroll
   for (int i = 0; i < G; ++i) u[i] = take(rows, i);
-  float scale = rows.slot != kNoSlot ? __ldg(scales + rows.slot) : 0.f;
-  uint32_t zero = FMT == GL_KV_INT4 && rows.slot != kNoSlot ? __ldg(zeros + rows.slot) : 0u;
+  float scale = rows.slot != kNoSlot ? kv_load(scales + rows.slot) : 0.f;
+  uint32_t zero = FMT == GL_KV_INT4 && rows.slot != kNoSlot ? kv_load(zeros + rows.slot) : 0u;
 
 #pragma unroll 1
   for (int n = 0; flags & 1u; ++n) {
@@ -314,8 +314,8 @@ __device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh
     flags = nxt.flags;
     rows = rows_next;
     if (flags & 1u) {
-      scale = rows.slot != kNoSlot ? __ldg(scales + rows.slot) : 0.f;
-      if (FMT == GL_KV_INT4) zero = rows.slot != kNoSlot ? __ldg(zeros + rows.slot) : 0u;
+      scale = rows.slot != kNoSlot ? kv_load(scales + rows.slot) : 0.f;
+      if (FMT == GL_KV_INT4) zero = rows.slot != kNoSlot ? kv_load(zeros + rows.slot) : 0u;
       nxt = fetch();
     }
   }

@@ -115,3 +115,38 @@ def test_norm_of_large_heads(lib, size):
     key = cache.read(table, _i32([3]), max_len=3, out_dtype=torch.float32)[0]
     scale = want[:, :1].abs().amax(-1, keepdim=True) / 127
     assert bool(((key[0, :2].double() - want[:, :1]).abs() <= 0.5 * scale * (1 + 2.0 ** -10)).all()) and bool(key[0, 2].isnan().all())
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("T,hq", [(1, 8), (4, 8), (24, 32), (150, 32)])
+@pytest.mark.parametrize("graph", [False, True])
+def test_overwritten_slots_are_read_anew(lib, fmt, T, hq, graph):
+    """write and attend in turn on the same slots, launched while the kernels before them still run: every attend sees what the
+    write before it left, as it does when each call is waited for."""
+    from gemlite_b200 import KVBatch
+    hkv, steps, ctx = 2, 30, 200
+    cache, table = make_cache([ctx + T] * 6, hkv, 128, fmt, 16, seed=40)
+    n = 6 * T
+    q, k, v = _randn(41, n, hq, 128), _randn(42, steps, n, hkv, 128), _randn(43, steps, n, hkv, 128)
+    batch = KVBatch(table, _i32([ctx] * 6), max_len=ctx + T, max_new=T)
+
+    def step(i):
+        cache.write(None, k[i], v[i], batch)
+        return cache.attend(q, batch)
+
+    want = []
+    for i in range(steps):
+        want.append(step(i))
+        torch.cuda.synchronize()
+    assert not torch.equal(want[0], want[1])
+    if graph:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            got = [step(i) for i in range(steps)]
+        g.replay()
+    else:
+        got = [step(i) for i in range(steps)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
