@@ -192,21 +192,23 @@ __device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh
   uint8_t* tiles = base + (values ? Lay<D>::V : Lay<D>::K);
 
   KvPiece pc;
-  bool have = walk.next(p, blockIdx.x, pc);
-  int tile = have ? pc.t0 : 0;
+  bool have;
+  int tile, parted;                                                       // parted: first tile that not every row of the unit sees all of
+  auto next_piece = [&]() {
+    have = walk.next(p, blockIdx.x, pc);
+    tile = have ? pc.t0 : 0;
+    parted = have ? (pc.s.ctx + (p.mask == nullptr ? pc.row0 / p.group + 1 : 0)) / kKvTile : 0;
+  };
+  next_piece();
   // A tile two ahead: its page numbers are on their way while the codes of the one before are fetched.
-  struct Item { int page, place, head; uint32_t flags; };                 // flags: 1 tile exists, 2 token within the sequence, 4 not all rows see all of it
+  struct Item { int page, place, head; uint32_t flags; };                 // flags: 1 tile exists, 2 token within the sequence, 4 parted
   auto fetch = [&]() {
     Item it{-1, 0, 0, 0u};
-    while (have && tile >= pc.t1) {
-      have = walk.next(p, blockIdx.x, pc);
-      tile = have ? pc.t0 : 0;
-    }
+    while (have && tile >= pc.t1) next_piece();
     if (have) {
       const int pos = tile * kKvTile + w * 32 + lane;
       it.head = pc.head;
-      const int seen = pc.s.ctx + (p.mask == nullptr ? pc.row0 / p.group + 1 : 0);      // by every row of the unit
-      it.flags = 1u | ((tile + 1) * kKvTile > seen ? 4u : 0u);
+      it.flags = 1u | (tile >= parted ? 4u : 0u);
       if (pos < pc.s.len) {
         const int pi = p.page_shift >= 0 ? pos >> p.page_shift : pos / kb.page_size;
         it.place = pos - pi * kb.page_size;
@@ -248,12 +250,12 @@ __device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh
 #pragma unroll 1
   for (int n = 0; flags & 1u; ++n) {
     const int st = n & 1;
-    const bool parted = flags & 4u;
+    const bool in_part = flags & 4u;
     // the power of two, and whether the scales are near enough to each other
     const uint32_t bits = __float_as_uint(scale);
     const bool plain = bits - 1u < 0x7f7fffffu;                          // positive and finite
     const uint32_t hi = __reduce_max_sync(0xffffffffu, plain ? bits : 0u), lo = __reduce_min_sync(0xffffffffu, plain ? bits : 0x7f7fffffu);
-    const bool apart = parted || (int)(hi >> 23) - (int)(lo >> 23) >= (values ? kSpreadV<FMT> : kSpread);
+    const bool apart = in_part || (int)(hi >> 23) - (int)(lo >> 23) >= (values ? kSpreadV<FMT> : kSpread);
     const int e = apart ? 0 : pow2_above(hi) - (values ? 0 : kRoom<FMT>);
     const bool number = fabsf(scale) < INFINITY, none = apart && scale < kTinyScale;
     const uint32_t valid = __ballot_sync(0xffffffffu, rows.slot != kNoSlot);
@@ -277,7 +279,7 @@ __device__ __forceinline__ void convert_role(const KvAttendParams& p, Shared& sh
 #pragma unroll
       for (int i = 0; i < G; ++i) {
         const int t = c_tok + (g + i) * C::TPI;
-        if (FMT == GL_KV_FP8 && values && parted) {
+        if (FMT == GL_KV_FP8 && values && in_part) {
           const uint32_t m = 0x7f7f7f7fu, one = 0x01010101u;
           const bool nan = (((((u[i].x & m) + one) | ((u[i].y & m) + one) | ((u[i].z & m) + one) | ((u[i].w & m) + one)) & 0x80808080u) != 0);
           const uint32_t who = __reduce_or_sync(0xffffffffu, nan ? 1u << t : 0u);
