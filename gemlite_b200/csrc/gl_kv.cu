@@ -17,6 +17,8 @@ int gl_kv_check(const char* fn, const gl_kv_args* a) {
     GL_FAIL(GL_E_UNSUPPORTED, "%s: %d pages of %d heads x %d tokens (at most 2^32 - 2 rows)", fn, a->num_pages, a->n_kv_heads, a->page_size);
   if (!a->k_codes || !a->v_codes || !a->k_scales || !a->v_scales) GL_FAIL(GL_E_INVALID, "%s: null cache pointer", fn);
   if (((uintptr_t)a->k_codes | (uintptr_t)a->v_codes) & 15) GL_FAIL(GL_E_INVALID, "%s: codes must be 16-byte aligned", fn);
+  if (((uintptr_t)a->k_scales | (uintptr_t)a->v_scales | (uintptr_t)a->page_table | (uintptr_t)a->lens | (uintptr_t)a->q_offsets) & 3)
+    GL_FAIL(GL_E_INVALID, "%s: scales, page table, lengths and offsets must be 4-byte aligned", fn);
   if (a->format == GL_KV_INT4 && (!a->k_zeros || !a->v_zeros)) GL_FAIL(GL_E_INVALID, "%s: the 4-bit cache needs zeros", fn);
   if (a->batch > 0 && (!a->lens || (a->max_pages > 0 && !a->page_table))) GL_FAIL(GL_E_INVALID, "%s: null page table or lengths", fn);
   if (a->batch > 0 && a->q_offsets == nullptr && a->n_tokens % a->batch != 0)
@@ -430,6 +432,8 @@ extern "C" int gl_kv_write(const gl_kv_args* a, void* stream) {
   if (a->rot_dim > 0 && ((uintptr_t)a->cos_sin & 15)) GL_FAIL(GL_E_INVALID, "gl_kv_write: the cos / sin table must be 16-byte aligned");
   if ((a->q_norm || a->k_norm) && a->norm_dtype != GL_FP32 && a->norm_dtype != GL_FP16 && a->norm_dtype != GL_BF16)
     GL_FAIL(GL_E_INVALID, "gl_kv_write: norm weights of dtype %d", a->norm_dtype);
+  if (((a->q_norm || a->k_norm) && (((uintptr_t)a->q_norm | (uintptr_t)a->k_norm) & (gl_dtype_size(a->norm_dtype) - 1))) || (a->rot_dim > 0 && ((uintptr_t)a->positions & 3)))
+    GL_FAIL(GL_E_INVALID, "gl_kv_write: misaligned norm weights or positions");
   WriteParams p;
   p.kb = gl_kv_batch(a);
   p.q = a->q; p.k = a->k; p.v = a->v; p.q_out = a->out;

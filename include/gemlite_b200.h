@@ -313,7 +313,7 @@ GL_API int gl_silu_mul(const void* gate_up, void* out, int32_t M, int32_t inter,
  * not depend on them.
  *
  * Pointers and strides: q / k / v [n_tokens, heads, head_dim], fp16 or bf16, 16-byte aligned, strides in elements and
- * multiples of 8, channels contiguous; outputs contiguous. */
+ * multiples of 8, channels contiguous; outputs contiguous.  All other pointers are aligned to their element. */
 enum { GL_KV_FP8 = 0, GL_KV_INT8 = 1, GL_KV_INT4 = 2 };
 typedef struct gl_kv_args {
   void*          k_codes;
