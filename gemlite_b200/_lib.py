@@ -96,6 +96,7 @@ SIGNATURES = {
     "gl_kv_read": (c_int32, [ctypes.POINTER(GLKvArgs), c_void_p]),
     "gl_kv_attend_workspace_bytes": (c_uint64, [ctypes.POINTER(GLKvArgs)]),
     "gl_kv_attend": (c_int32, [ctypes.POINTER(GLKvArgs), c_void_p]),
+    "gl_kv_attend_status": (c_int32, [ctypes.POINTER(c_int32), c_int32, c_void_p]),
     "gl_mma_peak": (c_int32, [c_int32, c_int32, c_void_p, ctypes.POINTER(ctypes.c_double), c_void_p]),
 }
 

@@ -32,6 +32,9 @@
 namespace {
 using namespace gltc;
 
+// 0, or what waits that gave up left since it was last cleared: 1 a wait of the roles, 2 the one before the TMEM goes back
+__device__ int g_wait_status;
+
 constexpr int kThreads = 20 * 32;             // 17 warps work; 20 fill the five warp groups that share out the registers
 constexpr int kMeta = 4;                       // tiles' scalars and masks: a tile's are read before the second tile after it is converted
 constexpr float kOff = 7.f, kRaise = 8.f;
@@ -716,7 +719,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tc_kernel(const KvAtten
   __syncthreads();
   tc_fence_after();
 
-  // Every wait is bounded; one that gives up ends all roles, and the rows that it leaves unfinished become NaN.
+  // Every wait is bounded; one that gives up ends all roles, the rows that it leaves unfinished become NaN, and the status says so.
   // Registers: 640 threads are launched with 96 each; 2 x 128 + 2 x 88 + 48 = 480 = 5 x 96 are shared out again.
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
@@ -737,6 +740,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tc_kernel(const KvAtten
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (threadIdx.x == 0 && (sh.abort | sh.never) != 0) atomicOr(&g_wait_status, sh.abort | sh.never << 1);
   if (warp == 16) tmem_dealloc(sh.tmem, 512);
 }
 
@@ -757,6 +761,21 @@ int launch_fmt(const KvAttendParams& p, int fmt, cudaStream_t st) {
 }
 
 }  // namespace
+
+extern "C" int gl_kv_attend_status(int32_t* status, int32_t clear, void* stream) {
+  if (status == nullptr) GL_FAIL(GL_E_INVALID, "gl_kv_attend_status: null argument");
+  cudaStream_t st = (cudaStream_t)stream;
+  int now = 0;
+  GL_CUDA_CHECK(cudaMemcpyFromSymbolAsync(&now, g_wait_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
+  GL_CUDA_CHECK(cudaStreamSynchronize(st));
+  *status = now;
+  if (now != 0 && clear) {
+    now = 0;
+    GL_CUDA_CHECK(cudaMemcpyToSymbolAsync(g_wait_status, &now, sizeof(int), 0, cudaMemcpyHostToDevice, st));
+    GL_CUDA_CHECK(cudaStreamSynchronize(st));
+  }
+  return GL_OK;
+}
 
 int gl_kv_attend_tc_launch(const KvAttendParams& p, int head_dim, int format, int x_dtype, cudaStream_t st) {
   if (head_dim == 128) return x_dtype == GL_BF16 ? launch_fmt<128, __nv_bfloat16>(p, format, st) : launch_fmt<128, __half>(p, format, st);

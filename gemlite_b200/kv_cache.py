@@ -45,6 +45,17 @@ def rotary_table(max_positions: int, rot_dim: int, base: float = 10000.0, device
     return torch.cat([angle.cos(), angle.sin()], 1).to(torch.float32)
 
 
+def attend_status(device=None, clear: bool = True) -> int:
+    """0, unless a bounded wait of the kernel for many rows gave up on `device` since the status was last cleared: the rows
+    that it left unfinished are NaN.  Synchronises the current stream."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    status = ctypes.c_int32()
+    with torch.cuda.device(device):
+        stream = torch.cuda.current_stream().cuda_stream
+        _lib.check(_lib.lib().gl_kv_attend_status(ctypes.byref(status), int(clear), stream))
+    return status.value
+
+
 def _index_tensor(t, what, dim):
     _lib.require_cuda(t, what)
     if t.dtype != torch.int32 or t.dim() != dim or (t.numel() > 0 and t.stride(-1) != 1 and t.shape[-1] > 1):

@@ -363,6 +363,11 @@ GL_API int gl_kv_read(const gl_kv_args* a, void* stream);
  * What a token does not see has no influence, whatever the bytes there hold. */
 GL_API uint64_t gl_kv_attend_workspace_bytes(const gl_kv_args* a);
 GL_API int gl_kv_attend(const gl_kv_args* a, void* stream);
+/* The waits inside the tcgen05 attention kernel are bounded; rows that one of them left unfinished when it gave up are NaN.
+ * Here the caller can tell such rows from a NaN of the cache's: 0 unless a wait gave up on the current device since the status
+ * was last cleared (on any stream; work on other streams counts once it has run).  Waits for `stream`; not for a
+ * stream that is being captured. */
+GL_API int gl_kv_attend_status(int32_t* status, int32_t clear, void* stream);
 
 /* ---- measurement: tensor-pipe ceiling ------------------------------------------------------------ */
 /* Enqueues one kernel in which every SM issues iters x 4 tcgen05.mma of 128 x 256 x (32 bytes of K) on operand tiles

@@ -150,3 +150,14 @@ def test_overwritten_slots_are_read_anew(lib, fmt, T, hq, graph):
         got = [step(i) for i in range(steps)]
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_status_after_clean_launches(lib):
+    """(A wait that runs out cannot be made on a GPU without work left in flight.)"""
+    from gemlite_b200 import KVBatch, kv_cache
+    cache, table = make_cache([300], 2, 128, "fp8", 16, seed=50)
+    out = cache.attend(_randn(51, 40, 16, 128), KVBatch(table, _i32([260])))
+    assert kv_cache.attend_status() == 0 == kv_cache.attend_status(DEV, clear=False) and bool(out.isfinite().all())
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        assert kv_cache.attend_status("cuda") == 0

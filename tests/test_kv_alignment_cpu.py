@@ -23,3 +23,9 @@ def test_write_operands(lib, bad):
     from gemlite_b200 import _lib
     assert lib.gl_kv_write(ctypes.byref(_args(**bad)), None) == _lib.GL_E_INVALID
     assert b"misaligned" in lib.gl_last_error()
+
+
+def test_status_needs_a_place_for_its_answer(lib):
+    from gemlite_b200 import _lib
+    assert lib.gl_kv_attend_status(None, 0, None) == _lib.GL_E_INVALID
+    assert b"gl_kv_attend_status" in lib.gl_last_error()
