@@ -161,3 +161,119 @@ def test_status_after_clean_launches(lib):
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
         assert kv_cache.attend_status("cuda") == 0
+
+
+# ---- many sequences, many rows -----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kernel,B", [(1, 129), (1, 700), (2, 641), (2, 1500)])
+def test_more_sequences_than_threads(lib, kernel, B):
+    """Where a thread that adds up the work takes several sequences."""
+    from gemlite_b200 import KVBatch
+    ctx, new = [(37 * i) % 211 for i in range(B)], [(i * 5) % 4 for i in range(B)]
+    ctx[B // 2] = 3000
+    cache, table = make_cache([c + t for c, t in zip(ctx, new)], 2, 64, "int8", 16, seed=60)
+    q = _randn(61, sum(new), 4, 64)
+    batch = KVBatch(table, _i32(ctx), _i32([0] + torch.tensor(new).cumsum(0).tolist()), max_len=3003, max_new=3)
+    _check_attend(cache, table, ctx, new, q, None, cache.attend(q, batch, kernel_override=kernel), rounds_codes=kernel == 2)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+def test_many_rows_repeat_streams_and_graphs(lib, masked):
+    """The tcgen05 kernel: the same call gives the same bits; two graphs and side streams share no scratch; a replay sees the lengths
+    that the tensors hold then."""
+    from gemlite_b200 import KVBatch
+    hq, hkv, T = 64, 8, 50
+    cache, table = make_cache([2000, 1200, 300], hkv, 128, "fp8", 16, seed=62)
+    ctx = _i32([1950, 600, 0])
+    q = _randn(63, 3 * T, hq, 128)
+    mask = torch.ones(T, T, dtype=torch.bool, device=DEV).tril().repeat(3, 1) if masked else None
+    batch = KVBatch(table, ctx)
+    want = cache.attend(q, batch, mask=mask)
+    assert all(torch.equal(cache.attend(q, batch, mask=mask), want) for _ in range(20))
+    side, graphs, outs = torch.cuda.Stream(), [], []
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            outs.append(cache.attend(q, batch, mask=mask))
+        graphs.append(g)
+    ctx.copy_(_i32([1000, 1100, 250]))
+    later = cache.attend(q, batch, mask=mask)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    eager = []
+    for _ in range(10):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(streams[2]):
+            eager.append(cache.attend(q, batch, mask=mask))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, later) for x in outs + eager) and not torch.equal(later, want)
+
+
+def test_long_cache_with_many_rows(lib):
+    """Codes of more than 4 GB under the tcgen05 kernel: pages at the far end."""
+    from gemlite_b200 import KVBatch, QuantizedKVCache
+    pages, ps, heads, T = 4300, 128, 64, 66
+    cache = QuantizedKVCache(pages, ps, heads, 128, "fp8", device=DEV)
+    assert cache.k_codes.numel() > 2 ** 32
+    table = torch.arange(pages - 2, pages, dtype=torch.int32, device=DEV)[None].contiguous()
+    k, v, q = _randn(1, 130, heads, 128), _randn(2, 130, heads, 128), _randn(3, T, heads, 128)
+    cache.write(None, k, v, KVBatch(table, _i32([0])))
+    out = cache.attend(q, KVBatch(table, _i32([130 - T])), kernel_override=2)
+    _check_attend(cache, table, [130 - T], [T], q, None, out, rounds_codes=True)
+
+
+# ---- what a write leaves, bit for bit ------------------------------------------------------------------------------------------
+def _codes32(x, fmt):
+    """Codes, scales and zero points of the rows of x (fp32, on the CPU) by the formulas, every operation rounded to fp32 by itself."""
+    if fmt == "int4":
+        lo, hi = x.amin(-1, keepdim=True).clamp(max=0), x.amax(-1, keepdim=True).clamp(min=0)
+        scale = ((hi - lo) / torch.full_like(lo, 15)).clamp(min=1e-6)
+        zero = (-lo / scale).round().clamp(0, 15)
+        c = ((x / scale).round() + zero).clamp(0, 15).to(torch.uint8)
+        return c[..., 0::2] | c[..., 1::2] << 4, scale[..., 0], zero[..., 0].to(torch.uint8)
+    top = 448.0 if fmt == "fp8" else 127.0
+    most = x.abs().amax(-1, keepdim=True)
+    scale = (most / torch.full_like(most, top)).clamp(min=1e-6)
+    c = (x / scale).clamp(-top, top)
+    c = c.to(torch.float8_e4m3fn).view(torch.uint8) if fmt == "fp8" else c.round().to(torch.int8).view(torch.uint8)
+    return c, scale[..., 0], None
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("d,hkv,dtype,inter", [(128, 8, torch.bfloat16, False), (64, 3, torch.float16, True)])
+def test_written_bits(lib, fmt, d, hkv, dtype, inter):
+    """Codes, scales and zero points equal those of the formulas in fp32 (the norm's sum of squares in fp64), and nobody's slots
+    keep all of theirs, zero points too."""
+    from gemlite_b200 import KVBatch, rotary_table
+    ctx, new, page = [0, 33, 70], [500, 1, 90], 16
+    cache, table = make_cache([c + t for c, t in zip(ctx, new)], hkv, d, fmt, page, seed=70)
+    names = ["k_codes", "v_codes", "k_scales", "v_scales"] + (["k_zeros", "v_zeros"] if fmt == "int4" else [])
+    want = {n: getattr(cache, n).cpu().clone() for n in names}
+    n = sum(new)
+    k, v = _randn(71, n, hkv, d, dtype=dtype, scale=2.0), _randn(72, n, hkv, d, dtype=dtype, scale=3.0)
+    w, cs = (1 + 0.3 * _randn(73, d, dtype=torch.float32)).to(dtype), rotary_table(700, d, device=DEV)
+    pos = torch.cat([torch.arange(c, c + t) for c, t in zip(ctx, new)])
+    cache.write(None, k, v, KVBatch(table, _i32(ctx), _i32([0] + torch.tensor(new).cumsum(0).tolist())), positions=pos.to(DEV), cos_sin=cs, k_norm=w,
+                eps=1e-5, interleaved=inter)
+
+    x = k.cpu().float()
+    mean = (x.double().square().sum(-1, keepdim=True) / d).float()
+    # (torch's CPU square root in fp32 is an ulp off for some arguments; through fp64 it is the correctly rounded one)
+    x = x * (torch.ones_like(mean) / (mean + 1e-5).double().sqrt().float()) * w.cpu().float()
+    t = cs.cpu()[pos][:, None]
+    cos, sin = t[..., :d // 2], t[..., d // 2:]
+    a, b = (x[..., 0::2], x[..., 1::2]) if inter else (x[..., :d // 2], x[..., d // 2:])
+    ra, rb = a * cos - b * sin, b * cos + a * sin
+    x = torch.stack([ra, rb], -1).flatten(-2) if inter else torch.cat([ra, rb], -1)
+    rows = torch.cat([torch.full((t,), b) for b, t in enumerate(new)])
+    pages, places = table.cpu()[rows, pos // page].long(), pos % page
+    for which, y in (("k", x), ("v", v.cpu().float())):
+        for name, value in zip(("_codes", "_scales", "_zeros"), _codes32(y, fmt)):
+            if value is not None:
+                want[which + name][pages, :, places] = value
+    for name in names:
+        got, ref = getattr(cache, name).cpu(), want[name]
+        as_bits = (lambda t: t.view(torch.int32)) if ref.dtype == torch.float32 else (lambda t: t)
+        assert torch.equal(as_bits(got), as_bits(ref)), (name, int((as_bits(got) != as_bits(ref)).sum()))
