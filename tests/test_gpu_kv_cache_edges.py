@@ -277,3 +277,26 @@ def test_written_bits(lib, fmt, d, hkv, dtype, inter):
         got, ref = getattr(cache, name).cpu(), want[name]
         as_bits = (lambda t: t.view(torch.int32)) if ref.dtype == torch.float32 else (lambda t: t)
         assert torch.equal(as_bits(got), as_bits(ref)), (name, int((as_bits(got) != as_bits(ref)).sum()))
+
+
+def test_compiled_layer_with_the_cache(lib):
+    """torch.compile breaks its graph at the cache's calls, which run as they do without it: same results, also when lengths,
+    buffers and batches change between calls."""
+    from gemlite_b200 import KVBatch, QuantizedKVCache, rotary_table, tp
+    layer = tp.LlamaLinears(512, 1024, 8, 2, 64, 1, 0, DEV, seed=3)
+    cs = rotary_table(64, 64, device=DEV)
+    compiled = torch.compile(layer, backend="eager")
+    caches = [make_cache([40, 9], 2, 64, "fp8", 16, seed=21)[0] for _ in range(2)]
+    table = make_cache([40, 9], 2, 64, "fp8", 16, seed=21)[1]
+    for i, (ctx, new) in enumerate((([36, 8], [4, 1]), ([30, 2], [1, 1]), ([0, 0], [9, 9]))):
+        n = sum(new)
+        x = _randn(80 + i, n, 512)
+        batch = KVBatch(table, _i32(ctx), _i32([0] + torch.tensor(new).cumsum(0).tolist()))
+        pos = torch.cat([torch.arange(c, c + t) for c, t in zip(ctx, new)]).to(DEV)
+        with torch.no_grad():
+            want = layer(x, caches[0], batch, positions=pos, cos_sin=cs)
+            got = compiled(x, caches[1], batch, positions=pos, cos_sin=cs)
+        assert torch.equal(got, want)
+        for name in ("k_codes", "v_codes", "k_scales", "v_scales"):
+            assert torch.equal(getattr(caches[0], name).view(torch.uint8), getattr(caches[1], name).view(torch.uint8))
+        caches[1].k_scales = caches[1].k_scales.clone()
