@@ -1,8 +1,9 @@
 // Quantised key/value cache: write (head norms, rotary positions and quantisation in one pass) and read back, sm_100a.
 //
-// Both kernels move bytes: every operand is read once with 16-byte loads, every output written once.  A row (one token's
-// head) is spread over head_dim / 8 lanes of 8 channels each, so that norms and maxima are three or four shuffles and the
-// rotation's partner channel is one.
+// Both kernels move bytes: every operand is read once, every output written once.  A row (one token's head) is spread over
+// head_dim / 8 lanes of 8 channels each, so that norms and maxima are three or four shuffles.  The write takes a lane's channels as
+// two pieces of 4 (8-byte loads), which puts both channels of a rotated pair into one lane; the read takes them as one piece of codes
+// (8 bytes, 4 in the 4-bit format) and stores 16 bytes or more of the output.
 #include "gl_kv_attend.cuh"
 
 int gl_kv_check(const char* fn, const gl_kv_args* a) {
@@ -68,7 +69,9 @@ struct WriteParams {
 //
 // 8192 tokens of 64 + 2 x 8 heads of 128 into fp8 (323 MB): 110 us, 2.9 TB/s (155 us with partners fetched by shuffles and one row
 // at a time).  Bound by issue slots (fp64 sums, correctly rounded divisions and roots) and by the latency of a token's loads;
-// 80 registers, three blocks per SM.  One token: 4.0 us, four dependent loads.
+// 80 registers (140 bytes of spills), three blocks per SM.  One token: 4.1 us, four dependent loads.  Fewer than 64 heads of 128 (128 of
+// 64) leave lane groups without a row that still go through the arithmetic: 3108 tokens of 24 + 2 x 4 heads of 64 into 4 bits (24 MB) take
+// 39 us under ncu.
 template <typename T, int LPR> struct Rows {
   static constexpr int D = LPR * 8;
   struct Raw { uint2 p, q; };
@@ -313,8 +316,8 @@ struct ReadParams {
 // One lane per 8 channels, so that a warp's stores are whole lines of the output; a block takes whole tokens (all heads of one
 // follow each other there).  Its rows' slots are looked up once, by one thread each, and every lane has the loads of eight rows, keys
 // and values, in flight.  Codes become fp16 numbers two at a time, exactly, and are scaled in fp32.
-// 95537 tokens of 8 heads of 128, int4 to bf16 (642 MB): 100 us, 6.4 TB/s, the measured copy bandwidth but for 2 % (four rows in flight:
-// 118 us; 16 channels per lane, whose stores fill half lines: 139 us).
+// 95537 tokens of 8 heads of 128, int4 to bf16 (642 MB): 100 us in a captured graph, 6.4 TB/s, the measured copy bandwidth but for 2 %;
+// 107 us (6.0 TB/s) called one by one (four rows in flight: 118 us captured; 16 channels per lane, whose stores fill half lines: 139 us).
 template <int D, int FMT, typename O>
 __global__ void __launch_bounds__(256) kv_read_kernel(const ReadParams p) {
   constexpr int RB = FMT == GL_KV_INT4 ? D / 2 : D, LPR = D / 8, GROUPS = 256 / LPR, N = 8, ROWS = GROUPS * N;

@@ -12,8 +12,9 @@
 // leaves the fp16 format 39 binary orders below the largest weight before a weight is lost.
 //
 // Bound by the cache's bytes, then by issue slots (conversion, about 500 instructions per 32 tokens of 128 channels).  32 decoding
-// sequences of 500 to 16000 tokens, 64 / 8 heads of 128 in fp8 (559 MB): 100 us, 5.6 TB/s.  One sequence of 131000 tokens, 8 / 1 heads,
-// int8 (35 MB): 20 us, of which the tokens take 5.
+// sequences of 500 to 16000 tokens, 64 / 8 heads of 128 in fp8 (559 MB): 100 us, 5.6 TB/s; 128 of 1000 to 8000 in fp8 (1.2 GB) 201 us,
+// 6.1 TB/s, in int4 (640 MB) 246 us, 2.6 TB/s: the 4-bit conversion (shift, mask, subtract, permute) is the bound there, not the bytes.  One
+// sequence of 131000 tokens, 8 / 1 heads, int8 (35 MB): 20 us, of which the tokens take 5.
 #include "gl_kv_attend.cuh"
 #include <mutex>
 
@@ -630,8 +631,12 @@ int launch_all(const KvAttendParams& p, const gl_kv_args* a, const Plan& pl, cud
   return pl.rows == 8 ? launch_join<8, D, T>(p, pl, st) : launch_join<16, D, T>(p, pl, st);
 }
 
-// Few rows per kv head: the mma.sync kernel, which holds 8 or 16 rows in registers; more: the
-// tcgen05 kernel with 256 (one per SM).
+// Few rows per kv head: the mma.sync kernel, which holds 8 or 16 rows in registers; more: the tcgen05 kernel with 256 (one block per SM).
+// 64 sequences of 500 to 4000 tokens, 8 kv heads of 128, us by mma.sync / tcgen05 at so many rows per kv head:
+//   fp8   8: 61 / 219   16: 83 / 230   24: 149 / 232   32: 154 / 233   40: 221 / 235   48: 228 / 240   64: 296 / 246   128: 591 / 279
+//   int4  8: 74 / 198   16: 106 / 208  24: 190 / 211   32: 193 / 214   40: 274 / 218   48: 280 / 223   64: 366 / 226   128: 713 / 260
+// Up to 32 rows (two passes over the codes) the first is faster in every format and head size; behind it 4 bits want the second, 8 bits
+// lose 6 % at 40 rows and gain 20 % at 64.
 Plan plan_of(const gl_kv_args* a) {
   Plan pl;
   const int group = a->n_q_heads / a->n_kv_heads;

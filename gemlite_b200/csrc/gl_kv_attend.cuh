@@ -61,7 +61,8 @@ constexpr int kKvTile = 128;
 // Starting and finishing a unit (queries, scratch or output, the pipeline's ends) costs as much as some tiles: they stand before
 // its tiles in the line, so that a block that gets many short units gets fewer tiles.  (Measured: 2 for units of 8 or 16 rows,
 // 106 us against 113 with 1 on 32 decoding sequences of 500 to 16000 tokens; 4 for units of 256, 329 us against 341 with 2 on 8
-// trees of 64.)
+// trees of 64.  The shortest calls pay for it: one token over 1000 cached took 9.6 us before there was a cost, 11.3 with it, because
+// the grid is sized by tiles alone and blocks that get only cost do nothing.)
 template <int ROWS> constexpr int kUnitCost = ROWS >= 256 ? 4 : 2;
 struct KvSeq {
   int first, new_b, ctx, len, tiles, blocks;      // blocks: row blocks per kv head (0: no new tokens); tiles: with the cost

@@ -25,7 +25,8 @@
 //
 // Bound by a stream's chain (scores, two passes over them, weights, products): a tile of 128 tokens takes about 7000 cycles where
 // the tensor pipe and the exponentials need about 2050 each.  8 trees of 64 tokens over 7000 to 16000, 64 / 8 heads of 128 in fp8
-// (193 GFLOP): 328 us, 588 TFLOP/s; 1000 tokens over 7000 (246 GFLOP): 398 us, 617 TFLOP/s.
+// (193 GFLOP): 327 us, 591 TFLOP/s; 1000 tokens over 7000 (246 GFLOP): 400 us, 614 TFLOP/s.  The compiler spills 268 bytes for heads of 128
+// and 84 for heads of 64, the same in every format and type.
 #include "gl_kv_attend.cuh"
 #include "gl_tc_common.cuh"
 

@@ -4,7 +4,7 @@ The low-bit layers leave decode bound by the bytes of the cache once contexts gr
 8 or 4 bits.  Three calls make the step between a fused qkv projection and the output projection::
 
     cache = QuantizedKVCache(num_pages, page_size, n_kv_heads, head_dim, kv_format="fp8", device="cuda:0")
-    batch = KVBatch(page_table, ctx_lens, q_offsets)             # which pages, how many tokens cached, which rows are new
+    batch = KVBatch(page_table, ctx_lens, q_offsets, max_new=1)  # which pages, how many tokens cached, which rows are new
     q = cache.write(q, k, v, batch, positions=pos, cos_sin=table, q_norm=wq, k_norm=wk)
     y = cache.attend(q, batch)                                   # or attend(q, batch, mask=tree_mask)
 
@@ -70,8 +70,10 @@ class KVBatch:
     ctx_lens [B] int32: tokens that the cache holds of it already.
     q_offsets [B + 1] int32: its new tokens are rows q_offsets[b] .. q_offsets[b + 1] of the call's operands (ascending,
     rows behind the last one belong to nobody); None: the rows divide evenly.
-    max_len / max_new: bounds, known to the host, of cached + new and of new tokens per sequence.  They shape launches;
-    results do not depend on them.  Default: what the table holds, and all rows.
+    max_len / max_new: bounds, known to the host, of cached + new and of new tokens per sequence.  They shape launches (with
+    q_offsets and without max_new, a batch of decoding sequences goes to the kernel for many rows, at three times the time);
+    results change with them only by the kernels' roundings and the order of sums, also where they are too small.
+    Default: what the table holds, and all rows.
     """
 
     def __init__(self, page_table: Tensor, ctx_lens: Tensor, q_offsets: Optional[Tensor] = None,

@@ -309,8 +309,8 @@ GL_API int gl_silu_mul(const void* gate_up, void* out, int32_t M, int32_t inter,
  * q_offsets[b] .. q_offsets[b+1] of the token-major operands (q_offsets NULL: n_tokens / batch rows each), its token p
  * lives in page page_table[b, p / page_size].  Rows behind the last sequence's are neither read nor written.  A page
  * number outside 0 .. num_pages - 1, or a token behind the table's last column, counts as absent: not written, not seen,
- * read as zeros.  max_len and max_new are bounds of the lengths that the host knows; they shape the launch, results do
- * not depend on them.
+ * read as zeros.  max_len and max_new are bounds of the lengths that the host knows; they shape the launch: results change with
+ * them only by the kernels' roundings and the order of sums.  gl_kv_attend takes tables of up to 2^30 tokens (max_pages * page_size).
  *
  * Pointers and strides: q / k / v [n_tokens, heads, head_dim], fp16 or bf16, 16-byte aligned, strides in elements and
  * multiples of 8, channels contiguous; outputs contiguous.  All other pointers are aligned to their element. */
